@@ -252,6 +252,98 @@ int smx_moe_layer_dev(smx_ctx* ctx, size_t layer, const float* xs_dev, size_t m,
                       size_t nplan, const int32_t* slot_tok, const float* wslot, size_t slots,
                       float* y_dev);
 
+/* ---- a paged key/value cache in 8 bits and the attention over it.  The reference's counterparts: qkv_post / rope kernels and
+ *      the cache append (crates/strix-backend-rocm/src/kernels.rs:1885-2111, 1239, 1754), sdpa and its split form (:1247-1288,
+ *      2114-2200, 2280-2589; decode.rs:5326-5368); there the cache is fp32 or f16 and contiguous.
+ *
+ *      The cache is the caller's memory: int8 codes and one fp32 scale for each block of SMX_KV_BLOCK tokens and key/value
+ *      head, in pages of page_tokens tokens (a multiple of SMX_KV_BLOCK) of every head.  A stored value is code * scale.
+ *      With dim64 = head_dim rounded up to 64 the planes are, slowest index first,
+ *          k        [page][head][block][token / 16][d / 64][d / 16 % 4][token % 16][d % 16]
+ *          v        [page][head][block][d / 32][token / 4 % 4][d % 16][d / 16 % 2][token / 16][token % 4]
+ *          scales   [page][head][block]
+ *      (what one matrix instruction takes from each lane is contiguous).  Codes and scales of tokens that no sequence holds
+ *      may be anything.  smx_kv_sizes gives the plane sizes; the code planes are 16-byte aligned. ---- */
+#define SMX_KV_BLOCK 32
+#define SMX_KV_MAX_HEAD_DIM 256
+#define SMX_TYPE_F32 0    /* element types, by their ggml numbers */
+#define SMX_TYPE_BF16 30
+typedef struct smx_kv_cache {
+    int8_t* k;
+    int8_t* v;
+    float* k_scale;
+    float* v_scale;
+    size_t pages, page_tokens, kv_heads, head_dim; /* head_dim: even, at most SMX_KV_MAX_HEAD_DIM */
+} smx_kv_cache;
+/* The rows of one step: row r of sequence s is the token at position len[s] - n_s + (r - row0[s]), n_s = row0[s + 1] - row0[s];
+ * len counts this step's rows in.  len, row0 and table are read on the device when the kernels run, so a captured graph serves
+ * every step whose values keep within rows, max_rows and max_len; what they exceed them by is left out, and page numbers
+ * outside the cache are clamped into it. */
+typedef struct smx_kv_batch {
+    size_t nseq;
+    const int32_t* len;    /* device [nseq] */
+    const int32_t* row0;   /* device [nseq + 1], ascending from 0; NULL: one row for each sequence */
+    const int32_t* table;  /* device [nseq][table_ld]: the page of each page_tokens tokens */
+    size_t table_ld;
+    size_t rows;           /* rows of all sequences (nseq when row0 is NULL) */
+    size_t max_rows;       /* at least every n_s (1 when row0 is NULL) */
+    size_t max_len;        /* at least every len */
+} smx_kv_batch;
+/* Position rotation of the first rot_dim (even) channels: (a, b) -> (a cos - b sin, a sin + b cos) with (a, b) channels
+ * (i, i + rot_dim / 2), or (2 i, 2 i + 1) when interleaved, and table[position][i] = {cos, sin} (fp32, device; positions from
+ * n_pos on take the last row).  Every product and sum is rounded to fp32 by itself. */
+typedef struct smx_rope {
+    const float* table; /* device [n_pos][rot_dim / 2][2] */
+    size_t n_pos, rot_dim;
+    int interleaved;
+} smx_rope;
+/* table[p][i] = cos, sin of p * base^(-2 i / rot_dim), formed in 64 bits. */
+int smx_rope_table_dev(smx_ctx* ctx, float base, size_t rot_dim, size_t n_pos, float* table_dev);
+/* Bytes of one code plane and floats of one scale plane. */
+int smx_kv_sizes(size_t pages, size_t page_tokens, size_t kv_heads, size_t head_dim, size_t* code_bytes, size_t* scales);
+/* Stores a step's keys (rotated, when rope is given) and values: k, v [rows][kv_heads][head_dim] of `type` with ldk, ldv elements
+ * from row to row.  With q, the queries [rows][q_heads][head_dim] are rotated the same way into q_out (which may be q).
+ * scale = largest |value| of the block / 127, 0 (and zero codes) where that is below 2^-96, code = round-half-even(value *
+ * (1 / scale)).  New tokens that join earlier ones in a block never lower its scale; where they raise it the earlier codes become
+ * round(code * (old / new)).  A block that receives a value that is not finite gets a NaN scale (until a new sequence starts it
+ * again).  Results do not depend on the launch; appending the same rows twice leaves what appending them once does. */
+int smx_kv_append_dev(smx_ctx* ctx, const smx_kv_cache* cache, const smx_kv_batch* batch, int type, const void* k_dev, size_t ldk,
+                      const void* v_dev, size_t ldv, const smx_rope* rope, const void* q_dev, size_t ldq, size_t q_heads,
+                      void* q_out_dev, size_t ldqo);
+/* The stored keys and values of the batch's rows as fp32 [rows][kv_heads][head_dim] (either may be NULL). */
+int smx_kv_read_dev(smx_ctx* ctx, const smx_kv_cache* cache, const smx_kv_batch* batch, float* k_dev, float* v_dev);
+/* out = softmax(scale * q K^T) V for each query row and head over the row's own sequence: keys at positions up to the row's own
+ * and, with window > 0, only the last `window` of them.  q, out: [rows][q_heads][head_dim] of `type`, ldq, ldo elements from row
+ * to row; q_heads a multiple of kv_heads, query heads of one group next to each other.  A row that sees no key gives zeros.
+ * fp32 rows are computed to fp32 accuracy (queries and probabilities as two f16 terms each on the matrix cores), bf16 rows with one
+ * f16 term; statistics and sums are fp32.  A row's result depends on its own sequence and on the sizes of the call (nseq, rows,
+ * max_rows, max_len, which set how a long sequence is split), not on the other sequences.  Capturable. */
+int smx_attn_dev(smx_ctx* ctx, const smx_kv_cache* cache, const smx_kv_batch* batch, int type, const void* q_dev, size_t ldq,
+                 size_t q_heads, float scale, size_t window, void* out_dev, size_t ldo);
+
+/* ---- one token for each row of logits from given uniform numbers (the reference picks greedily: lm_head_argmax_rows).
+ *      Per row, with x the logits (NaN and -inf are never picked; entries equal to a +inf maximum share it) and m their maximum:
+ *        temperature T > 0: e_i = exp((x_i - m) / T) in fp32 and the whole-number weight w_i = floor(e_i * 2^40); T <= 0: the
+ *                    largest logit, lowest index on equal ones
+ *        top_k > 0:  the k first in (logit descending, index ascending) order stay
+ *        top_p < 1:  of those, the ones with less than floor(top_p * their total) in front of them in that order stay, and the first
+ *        min_p > 0:  of those, the ones with e_i >= min_p stay
+ *        the pick is the lowest index whose running total of kept weights (in index order) exceeds floor(u * their total)
+ *      All sums are of whole numbers, so a pick does not depend on how the work is split.  u in [0, 1). ---- */
+typedef struct smx_sample_params { /* device arrays [rows]; NULL: 1, off, off, off for every row */
+    const float* temperature;
+    const int32_t* top_k;
+    const float* top_p;
+    const float* min_p;
+} smx_sample_params;
+/* logits [rows][vocab], ld elements from row to row; ids[rows]; prob (may be NULL): the pick's share of the kept weight.  A row
+ * without a finite or +inf logit gives id 0 and prob 0.  Capturable. */
+int smx_sample_dev(smx_ctx* ctx, const float* logits_dev, size_t rows, size_t vocab, size_t ld, const smx_sample_params* params,
+                   const float* u_dev, int32_t* ids_dev, float* prob_dev);
+/* smx_lm_head_argmax_rows with the sampler in the place of the argmax: host buffers, params' arrays and u in host memory, one sync. */
+int smx_lm_head_sample_rows(smx_ctx* ctx, const char* key, const float* xs, size_t m, size_t in_dim, const smx_sample_params* params,
+                            const float* u, int32_t* out, float* prob);
+
 /* ---- HIP graph capture of a sequence of `_dev` calls: the role of the reference's captured decode
  *      token (decode.rs:3053-3203), so a launch-bound chain of small GEMVs replays without per-launch
  *      host cost.  Between begin and end only `_dev` entry points may be called, with shapes already

@@ -40,14 +40,64 @@ EXPORTS = [
     "smx_host_quantize_q8_0", "smx_host_quantize_q4_0", "smx_host_dequantize", "smx_moe_layer_dev",
     "smx_weight_dims", "smx_moe_layer_stages", "smx_gemv_noalloc_dev",
     "smx_gemv_f32", "smx_gemv_f32_dev", "smx_gemv_f32_batch", "smx_moe_route_dev", "smx_moe_route", "smx_moe_ffn_routed_dev", "smx_moe_router_dev", "smx_moe_ffn_logits_dev",
+    "smx_rope_table_dev", "smx_kv_sizes", "smx_kv_append_dev", "smx_kv_read_dev", "smx_attn_dev", "smx_sample_dev", "smx_lm_head_sample_rows",
 ]
 ACT_NONE, ACT_RMSNORM, ACT_SILU_MUL, ACT_GEGLU = 0, 1, 2, 3
+KV_BLOCK = 32                      # tokens of the cache that share a scale
+DTYPE_F32, DTYPE_BF16 = 0, 30      # element types of the cache's and attention's rows (ggml numbers)
 
 
 class SmxError(RuntimeError):
     def __init__(self, code, msg):
         super().__init__(f"smx error {code}: {msg}")
         self.code = code
+
+
+class _Struct(C.Structure):
+    """A structure of the C ABI that a program makes once and passes to many calls."""
+
+    @property
+    def addr(self):
+        return C.addressof(self)
+
+
+class _SampleParams(C.Structure):
+    _fields_ = [("temperature", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p), ("min_p", C.c_void_p)]
+
+
+class KvCache(_Struct):
+    """A paged int8 key/value cache of one layer in device memory of the caller's (smx_kv_cache; layout there)."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p), ("pages", C.c_size_t),
+                ("page_tokens", C.c_size_t), ("kv_heads", C.c_size_t), ("head_dim", C.c_size_t)]
+
+    def __init__(self, pages, page_tokens, kv_heads, head_dim, k, v, k_scale, v_scale):
+        super().__init__(k, v, k_scale, v_scale, pages, page_tokens, kv_heads, head_dim)
+
+
+class KvBatch(_Struct):
+    """The rows of one step (smx_kv_batch): lengths, page table and first rows are device arrays."""
+    _fields_ = [("nseq", C.c_size_t), ("len", C.c_void_p), ("row0", C.c_void_p), ("table", C.c_void_p), ("table_ld", C.c_size_t),
+                ("rows", C.c_size_t), ("max_rows", C.c_size_t), ("max_len", C.c_size_t)]
+
+    def __init__(self, nseq, len, table, table_ld, max_len, row0=None, rows=None, max_rows=None):
+        rows = nseq if rows is None else rows
+        super().__init__(nseq, len, row0, table, table_ld, rows, (1 if row0 is None else rows) if max_rows is None else max_rows, max_len)
+
+
+class Rope(_Struct):
+    """Position rotation (smx_rope): table[n_pos][rot_dim / 2][2] of fp32 cos, sin on the device."""
+    _fields_ = [("table", C.c_void_p), ("n_pos", C.c_size_t), ("rot_dim", C.c_size_t), ("interleaved", C.c_int)]
+
+    def __init__(self, table, n_pos, rot_dim, interleaved=False):
+        super().__init__(table, n_pos, rot_dim, 1 if interleaved else 0)
+
+
+def kv_sizes(pages, page_tokens, kv_heads, head_dim):
+    """(bytes of one code plane, floats of one scale plane) of a cache."""
+    nb, ns = C.c_size_t(), C.c_size_t()
+    if load_library().smx_kv_sizes(pages, page_tokens, kv_heads, head_dim, C.byref(nb), C.byref(ns)) != SMX_OK:
+        raise ValueError(f"no cache of {pages} pages of {page_tokens} tokens, {kv_heads} heads of {head_dim} channels")
+    return nb.value, ns.value
 
 
 _lib = None
@@ -149,6 +199,13 @@ def load_library():
     L.smx_host_quantize_q4_0.argtypes = [vp, sz, vp]
     L.smx_host_dequantize.argtypes = [i, vp, sz, vp]
     L.smx_gguf_upload_as.argtypes = [vp, vp, C.c_char_p, C.c_char_p, i]
+    L.smx_rope_table_dev.argtypes = [vp, C.c_float, sz, sz, vp]
+    L.smx_kv_sizes.argtypes = [sz, sz, sz, sz, C.POINTER(sz), C.POINTER(sz)]
+    L.smx_kv_append_dev.argtypes = [vp, vp, vp, i, vp, sz, vp, sz, vp, vp, sz, sz, vp, sz]
+    L.smx_kv_read_dev.argtypes = [vp, vp, vp, vp, vp]
+    L.smx_attn_dev.argtypes = [vp, vp, vp, i, vp, sz, sz, C.c_float, sz, vp, sz]
+    L.smx_sample_dev.argtypes = [vp, vp, sz, sz, sz, C.POINTER(_SampleParams), vp, vp, vp]
+    L.smx_lm_head_sample_rows.argtypes = [vp, cp, vp, sz, sz, C.POINTER(_SampleParams), vp, vp, vp]
     _lib = L
     return L
 
@@ -209,6 +266,18 @@ class CtypesCalls:
 
     def moe_ffn_routed_dev(self, c, layer, ids, w, k, x, y):
         return self._L.smx_moe_ffn_routed_dev(c, int(layer), ids, w, int(k), x, y)
+
+    def kv_append_dev(self, c, *a):
+        return self._L.smx_kv_append_dev(c, *a)
+
+    def kv_read_dev(self, c, *a):
+        return self._L.smx_kv_read_dev(c, *a)
+
+    def attn_dev(self, c, cache, batch, ty, q, ldq, q_heads, scale, window, out, ldo):
+        return self._L.smx_attn_dev(c, cache, batch, ty, q, ldq, q_heads, float(scale), window, out, ldo)
+
+    def sample_dev(self, c, logits, rows, vocab, ld, temperature, top_k, top_p, min_p, u, ids, prob):
+        return self._L.smx_sample_dev(c, logits, rows, vocab, ld, C.byref(_SampleParams(temperature, top_k, top_p, min_p)), u, ids, prob)
 
     def graph_launch(self, c, g):
         return self._L.smx_graph_launch(c, g)
@@ -687,6 +756,44 @@ class Mi355WeightAccel:
     def moe_shexp_dev(self, layer, sgate, x_dev, y_dev):
         """y_dev += sgate * shared_expert(x_dev) (decode.rs:1820-1855)."""
         return self._check(self._L.smx_moe_shexp_dev(self._h, layer, float(sgate), x_dev, y_dev))
+
+    # -- key/value cache, attention, sampling
+    def rope_table_dev(self, base, rot_dim, n_pos, table_dev):
+        self._check(self._L.smx_rope_table_dev(self._h, float(base), rot_dim, n_pos, table_dev))
+
+    def kv_append_dev(self, cache, batch, k, v, rope=None, q=None, q_heads=0, q_out=None, dtype=DTYPE_F32, ldk=None, ldv=None, ldq=None,
+                      ldqo=None):
+        """Keys (rotated) and values of a step's rows into the cache, its queries rotated into q_out (see smx_kv_append_dev).  ld*: elements
+        from row to row (default: rows without gaps)."""
+        w, qw = cache.kv_heads * cache.head_dim, q_heads * cache.head_dim
+        self._check(self._n.kv_append_dev(self._a, cache.addr, batch.addr, dtype, k, w if ldk is None else ldk, v, w if ldv is None else ldv,
+                                          None if rope is None else rope.addr, q, qw if ldq is None else ldq, q_heads, q_out,
+                                          qw if ldqo is None else ldqo))
+
+    def kv_read_dev(self, cache, batch, k_out, v_out):
+        """The stored keys and values of the batch's rows as fp32 (see smx_kv_read_dev)."""
+        self._check(self._n.kv_read_dev(self._a, cache.addr, batch.addr, k_out, v_out))
+
+    def attn_dev(self, cache, batch, q, q_heads, scale, out, window=0, dtype=DTYPE_F32, ldq=None, ldo=None):
+        """Attention of a step's query rows over the cache (see smx_attn_dev)."""
+        w = q_heads * cache.head_dim
+        self._check(self._n.attn_dev(self._a, cache.addr, batch.addr, dtype, q, w if ldq is None else ldq, q_heads, scale, window, out,
+                                     w if ldo is None else ldo))
+
+    def sample_dev(self, logits, rows, vocab, u, ids, temperature=None, top_k=None, top_p=None, min_p=None, prob=None, ld=None):
+        """One token for each row of logits; the parameters are device arrays, one value a row (see smx_sample_dev)."""
+        self._check(self._n.sample_dev(self._a, logits, rows, vocab, vocab if ld is None else ld, temperature, top_k, top_p, min_p, u, ids, prob))
+
+    def lm_head_sample_rows(self, key, xs, m, u, temperature=None, top_k=None, top_p=None, min_p=None):
+        """(ids, probabilities) of m rows through the lm_head and the sampler, or None when the key is not resident; host arrays."""
+        xs = _c(xs, np.float32).reshape(m, -1)
+        arrays = [None if a is None else _c(np.broadcast_to(a, m), t) for a, t in
+                  ((temperature, np.float32), (top_k, np.int32), (top_p, np.float32), (min_p, np.float32))]
+        u = _c(np.broadcast_to(u, m), np.float32)
+        ids, prob = np.empty(m, np.uint32), np.empty(m, np.float32)
+        params = _SampleParams(*(_p(a) for a in arrays))
+        ok = self._check(self._L.smx_lm_head_sample_rows(self._h, key.encode(), _p(xs), m, xs.shape[1], C.byref(params), _p(u), _p(ids), _p(prob)))
+        return (ids, prob) if ok else None
 
     def graph_begin(self):
         self._check(self._L.smx_graph_begin(self._h))

@@ -345,6 +345,22 @@ int smx_gemv_f32_batch(smx_ctx* c, size_t n, const char* const* keys, const floa
     return gemv_batch_host(c, n, keys, xs, in_lens, ys, out_caps, status, true);
 }
 
+// The rows of a host-pointer lm_head call to logits at c->yf32 (enqueued).  Rows of up to 8 MiB in all travel through the pinned
+// staging (a copy from pageable memory has the host wait for it); kernels that read a row once take it from the staging.
+static int lm_head_logits(smx_ctx* c, const Weight& w, const float* xs, size_t m) {
+    int rc;
+    const size_t xb = m * w.K * 4;
+    const bool pinned = xb <= (size_t(8) << 20);
+    if (pinned) {
+        if ((rc = ensure_host(c, c->hx, xb)) != SMX_OK) return rc;
+        memcpy(c->hx.p, xs, xb);
+    }
+    const bool direct = pinned && !(m <= 4 && !skinny_serves(w, m));
+    if (!pinned) SMX_HIP(c, hipMemcpyAsync(c->xf32.p, xs, xb, hipMemcpyHostToDevice, c->stream));
+    else if (!direct && (rc = staged_to_device(c, c->xf32.p, c->hx.p, xb)) != SMX_OK) return rc;
+    return run_matmul_dev(c, w, direct ? (const float*)c->hx.p : (const float*)c->xf32.p, m, (float*)c->yf32.p, false, nullptr, nullptr);
+}
+
 int smx_lm_head_argmax_rows(smx_ctx* c, const char* key, const float* xs, size_t m, size_t in_dim, uint32_t* out) {
     if (!c) return SMX_ERR_ARG;
     if (!key || !xs || !out) return fail(c, SMX_ERR_ARG, "lm_head_argmax_rows: null argument");
@@ -358,26 +374,57 @@ int smx_lm_head_argmax_rows(smx_ctx* c, const char* key, const float* xs, size_t
     if ((rc = ensure(c, c->xf32, m * w->K * 4)) != SMX_OK) return rc;
     if ((rc = ensure(c, c->yf32, m * w->N * 4)) != SMX_OK) return rc;
     if ((rc = ensure(c, c->tab, argmax_scratch_bytes(m, w->N))) != SMX_OK) return rc;   // the chunk candidates
-    // rows of up to 8 MiB in all travel through the pinned staging (a copy from pageable memory has the host wait for it),
-    // and the last kernel writes the indices into pinned memory itself
-    const size_t xb = m * w->K * 4;
-    const bool pinned = xb <= (size_t(8) << 20);
-    if (pinned) {
-        if ((rc = ensure_host(c, c->hx, xb)) != SMX_OK) return rc;
-        memcpy(c->hx.p, xs, xb);
-    }
+    // the last kernel writes the indices into pinned memory itself
     if ((rc = ensure_host(c, c->hy, m * 4)) != SMX_OK) return rc;
-    // (kernels that read a row once take it from the staging)
     HostCall call(c);
-    const bool direct = pinned && !(m <= 4 && !skinny_serves(*w, m));
-    if (!pinned) SMX_HIP(c, hipMemcpyAsync(c->xf32.p, xs, xb, hipMemcpyHostToDevice, c->stream));
-    else if (!direct && (rc = staged_to_device(c, c->xf32.p, c->hx.p, xb)) != SMX_OK) return rc;
-    rc = run_matmul_dev(c, *w, direct ? (const float*)c->hx.p : (const float*)c->xf32.p, m, (float*)c->yf32.p, false, nullptr, nullptr);
-    if (rc != SMX_OK) return rc;
+    if ((rc = lm_head_logits(c, *w, xs, m)) != SMX_OK) return rc;
     rc = launch_argmax_rows(c, (const float*)c->yf32.p, m, w->N, c->tab.p, (unsigned*)c->hy.p);
     if (rc != SMX_OK) return rc;
     if ((rc = stream_wait(c)) != SMX_OK) return rc;
     memcpy(out, c->hy.p, m * 4);
+    return call.done();
+}
+
+int smx_lm_head_sample_rows(smx_ctx* c, const char* key, const float* xs, size_t m, size_t in_dim, const smx_sample_params* params, const float* u,
+                            int32_t* out, float* prob) {
+    if (!c) return SMX_ERR_ARG;
+    if (!key || !xs || !u || !out) return fail(c, SMX_ERR_ARG, "lm_head_sample_rows: null argument");
+    const Weight* w = find_weight(c, key);
+    if (!w) return SMX_NOT_RESIDENT;
+    if (in_dim != w->K) return fail(c, SMX_ERR_ARG, "lm_head_sample_rows: activation length %zu, in_dim %zu", in_dim, w->K);
+    if (m == 0) return fail(c, SMX_ERR_ARG, "lm_head_sample_rows: zero rows");
+    int rc;
+    if ((rc = refuse_capture(c, "lm_head_sample_rows")) != SMX_OK) return rc;
+    SMX_HIP(c, hipSetDevice(c->device));
+    if ((rc = ensure(c, c->xf32, m * w->K * 4)) != SMX_OK) return rc;
+    if ((rc = ensure(c, c->yf32, m * w->N * 4)) != SMX_OK) return rc;
+    // pinned: picks, their probabilities, and the five words of each row that the sampler reads in place
+    if ((rc = ensure_host(c, c->hy, m * 7 * 4)) != SMX_OK) return rc;
+    int32_t* ids = (int32_t*)c->hy.p;
+    float* pr = (float*)(ids + m);
+    char* at = (char*)(pr + m);
+    auto put = [&](const void* a) -> void* {
+        void* to = at;
+        if (!a) return nullptr;
+        memcpy(to, a, m * 4);
+        at += m * 4;
+        return to;
+    };
+    smx_sample_params p = {};
+    const float* uu = (const float*)put(u);
+    if (params) {
+        p.temperature = (const float*)put(params->temperature);
+        p.top_k = (const int32_t*)put(params->top_k);
+        p.top_p = (const float*)put(params->top_p);
+        p.min_p = (const float*)put(params->min_p);
+    }
+    HostCall call(c);
+    if ((rc = lm_head_logits(c, *w, xs, m)) != SMX_OK) return rc;
+    if (w->N > (size_t(1) << 22)) return fail(c, SMX_ERR_LIMIT, "lm_head_sample_rows: %zu tokens (2^22)", w->N);
+    if ((rc = launch_sample(c, (const float*)c->yf32.p, m, w->N, w->N, &p, uu, ids, pr)) != SMX_OK) return rc;
+    if ((rc = stream_wait(c)) != SMX_OK) return rc;
+    memcpy(out, ids, m * 4);
+    if (prob) memcpy(prob, pr, m * 4);
     return call.done();
 }
 

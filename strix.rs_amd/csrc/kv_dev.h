@@ -1,0 +1,75 @@
+// The paged 8-bit key/value cache as the kernels see it (layout: smx_kv_cache in strix_mi355.h).
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "smx_internal.h"
+
+namespace smx {
+
+// Cache and batch of a launch, by value.
+struct KvArgs {
+    int8_t* k;
+    int8_t* v;
+    float* ks;
+    float* vs;
+    const int32_t* len;
+    const int32_t* row0;   // null: one row for each sequence
+    const int32_t* table;
+    int table_ld, pages, page_blocks, kv_heads, dim, dim64;
+    int nseq, rows, max_rows, max_len;
+};
+
+// One sequence of the batch: its rows [row, row + n) and the tokens [0, len) it holds; row j is the token len - n + j.
+struct KvSeq {
+    int row, n, len;
+};
+__device__ __forceinline__ KvSeq kv_seq(const KvArgs& a, int s) {
+    KvSeq q;
+    q.len = min(max(a.len[s], 0), a.max_len);
+    if (a.row0) {
+        const int r0 = min(max(a.row0[s], 0), a.rows), r1 = min(max(a.row0[s + 1], r0), a.rows);
+        q.row = r0;
+        q.n = min(r1 - r0, a.max_rows);
+    } else {
+        q.row = s;
+        q.n = 1;
+    }
+    return q;
+}
+// Index of a head's block `blk` (of SMX_KV_BLOCK tokens) of sequence s among all blocks of the cache.
+__device__ __forceinline__ int64_t kv_block(const KvArgs& a, int s, int head, int blk) {
+    const int p = blk / a.page_blocks;
+    const int page = min(max(a.table[(int64_t)s * a.table_ld + min(p, a.table_ld - 1)], 0), a.pages - 1);
+    return ((int64_t)page * a.kv_heads + head) * a.page_blocks + (blk - p * a.page_blocks);
+}
+// Byte of (token, channel) inside a block's keys / values.
+__device__ __forceinline__ int kv_k_byte(int dim64, int t, int d) {
+    return ((t >> 4) * (dim64 >> 6) + (d >> 6)) * 1024 + ((d >> 4) & 3) * 256 + (t & 15) * 16 + (d & 15);
+}
+__device__ __forceinline__ int kv_v_byte(int t, int d) {
+    return (d >> 5) * 1024 + ((t >> 2) & 3) * 256 + (d & 15) * 16 + ((d >> 4) & 1) * 8 + (t >> 4) * 4 + (t & 3);
+}
+
+__device__ __forceinline__ float bf16_to_f32(uint16_t h) { return __uint_as_float((unsigned)h << 16); }
+// round to nearest, ties to even; NaN stays NaN
+__device__ __forceinline__ uint16_t f32_to_bf16(float f) {
+    const unsigned u = __float_as_uint(f);
+    if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)((u >> 16) | 0x40);
+    return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
+}
+template <bool BF16>
+__device__ __forceinline__ float load_elem(const void* p, int64_t i) {
+    return BF16 ? bf16_to_f32(((const uint16_t*)p)[i]) : ((const float*)p)[i];
+}
+template <bool BF16>
+__device__ __forceinline__ void store_elem(void* p, int64_t i, float v) {
+    if (BF16) ((uint16_t*)p)[i] = f32_to_bf16(v);
+    else ((float*)p)[i] = v;
+}
+
+// Host side: the checks that every call over a cache makes, and the launch form of its arguments.
+int kv_args(smx_ctx* c, const char* who, const smx_kv_cache* cache, const smx_kv_batch* batch, KvArgs* out);
+
+}  // namespace smx

@@ -313,6 +313,9 @@ int launch_gemv_group(smx_ctx* c, const Weight* const* ws, const float* const* x
 int launch_gemv_dual(smx_ctx* c, const Weight* const* wg, const Weight* const* wu, const float* const* xs, float* const* yg,
                      float* const* yu, float* const* hs, int npairs, int act2, const ActProd* prod, const char* name, bool* served,
                      const GemvIndirect* ind = nullptr);
+// Sampling of device rows (sample.hip); the arrays of p, u, ids and prob are the device's (pinned host memory will do).
+int launch_sample(smx_ctx* c, const float* logits, size_t rows, size_t vocab, size_t ld, const smx_sample_params* p, const float* u, int32_t* ids,
+                  float* prob);
 // GEMM: y[m][N] on int8 MFMA.  dump (optional): out[m][N][K/32] i32.
 int launch_gemm(smx_ctx* c, const Weight& w, const int8_t* xq, const float* xd, size_t m, float* y,
                 int32_t* dump);

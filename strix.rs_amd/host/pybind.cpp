@@ -196,6 +196,37 @@ FN(moe_ffn_routed_dev) {
         !to_ptr(a[5], &x) || !to_ptr(a[6], &y)) return nullptr;
     ALLOW(smx_moe_ffn_routed_dev(c, layer, ids, w, k, x, y));
 }
+// (ctx, cache, batch, type, k, ldk, v, ldv, rope, q, ldq, q_heads, q_out, ldqo): cache, batch and rope are the structures' addresses
+FN(kv_append_dev) {
+    smx_ctx* c; const smx_kv_cache* cache; const smx_kv_batch* batch; const smx_rope* rope; int type; const void *k, *v, *q; void* qo;
+    size_t ldk, ldv, ldq, qh, ldqo;
+    if (!argc_is(n, 14) || !to_ptr(a[0], &c) || !to_ptr(a[1], &cache) || !to_ptr(a[2], &batch) || !to_int(a[3], &type) || !to_ptr(a[4], &k) ||
+        !to_size(a[5], &ldk) || !to_ptr(a[6], &v) || !to_size(a[7], &ldv) || !to_ptr(a[8], &rope) || !to_ptr(a[9], &q) || !to_size(a[10], &ldq) ||
+        !to_size(a[11], &qh) || !to_ptr(a[12], &qo) || !to_size(a[13], &ldqo)) return nullptr;
+    ALLOW(smx_kv_append_dev(c, cache, batch, type, k, ldk, v, ldv, rope, q, ldq, qh, qo, ldqo));
+}
+// (ctx, cache, batch, k_out, v_out)
+FN(kv_read_dev) {
+    smx_ctx* c; const smx_kv_cache* cache; const smx_kv_batch* batch; float *k, *v;
+    if (!argc_is(n, 5) || !to_ptr(a[0], &c) || !to_ptr(a[1], &cache) || !to_ptr(a[2], &batch) || !to_ptr(a[3], &k) || !to_ptr(a[4], &v)) return nullptr;
+    ALLOW(smx_kv_read_dev(c, cache, batch, k, v));
+}
+// (ctx, cache, batch, type, q, ldq, q_heads, scale, window, out, ldo)
+FN(attn_dev) {
+    smx_ctx* c; const smx_kv_cache* cache; const smx_kv_batch* batch; int type; const void* q; void* out; size_t ldq, qh, window, ldo; float scale;
+    if (!argc_is(n, 11) || !to_ptr(a[0], &c) || !to_ptr(a[1], &cache) || !to_ptr(a[2], &batch) || !to_int(a[3], &type) || !to_ptr(a[4], &q) ||
+        !to_size(a[5], &ldq) || !to_size(a[6], &qh) || !to_float(a[7], &scale) || !to_size(a[8], &window) || !to_ptr(a[9], &out) || !to_size(a[10], &ldo))
+        return nullptr;
+    ALLOW(smx_attn_dev(c, cache, batch, type, q, ldq, qh, scale, window, out, ldo));
+}
+// (ctx, logits, rows, vocab, ld, temperature, top_k, top_p, min_p, u, ids, prob)
+FN(sample_dev) {
+    smx_ctx* c; const float *x, *u; size_t rows, vocab, ld; smx_sample_params p; int32_t* ids; float* prob;
+    if (!argc_is(n, 12) || !to_ptr(a[0], &c) || !to_ptr(a[1], &x) || !to_size(a[2], &rows) || !to_size(a[3], &vocab) || !to_size(a[4], &ld) ||
+        !to_ptr(a[5], &p.temperature) || !to_ptr(a[6], &p.top_k) || !to_ptr(a[7], &p.top_p) || !to_ptr(a[8], &p.min_p) || !to_ptr(a[9], &u) ||
+        !to_ptr(a[10], &ids) || !to_ptr(a[11], &prob)) return nullptr;
+    ALLOW(smx_sample_dev(c, x, rows, vocab, ld, &p, u, ids, prob));
+}
 // (ctx, graph)
 FN(graph_launch) {
     smx_ctx* c; smx_graph* g;
@@ -296,7 +327,8 @@ PyMethodDef methods[] = {
     M("moe_ffn_logits_dev", moe_ffn_logits_dev), M("moe_ffn_routed_dev", moe_ffn_routed_dev), M("graph_launch", graph_launch),
     M("gemv", gemv_host<smx_gemv>), M("gemv_f32", gemv_host<smx_gemv_f32>), M("gemv_rows", rows_host<smx_gemv_rows>), M("gemm", rows_host<smx_gemm>),
     M("lm_head_argmax_rows", lm_head_argmax_rows), M("gemv_batch", gemv_batch), M("moe_ffn", moe_ffn), M("moe_ffn_dev", moe_ffn_dev),
-    M("moe_layer_dev", moe_layer_dev), M("moe_layer", moe_layer), {nullptr, nullptr, 0, nullptr}};
+    M("moe_layer_dev", moe_layer_dev), M("moe_layer", moe_layer),
+    M("kv_append_dev", kv_append_dev), M("kv_read_dev", kv_read_dev), M("attn_dev", attn_dev), M("sample_dev", sample_dev), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_smx_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
