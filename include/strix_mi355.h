@@ -330,6 +330,7 @@ int smx_attn_dev(smx_ctx* ctx, const smx_kv_cache* cache, const smx_kv_batch* ba
  *        min_p > 0:  of those, the ones with e_i >= min_p stay
  *        the pick is the lowest index whose running total of kept weights (in index order) exceeds floor(u * their total)
  *      All sums are of whole numbers, so a pick does not depend on how the work is split.  u in [0, 1). ---- */
+#define SMX_SAMPLE_MAX_VOCAB 2097152
 typedef struct smx_sample_params { /* device arrays [rows]; NULL: 1, off, off, off for every row */
     const float* temperature;
     const int32_t* top_k;

@@ -393,6 +393,7 @@ int smx_lm_head_sample_rows(smx_ctx* c, const char* key, const float* xs, size_t
     if (!w) return SMX_NOT_RESIDENT;
     if (in_dim != w->K) return fail(c, SMX_ERR_ARG, "lm_head_sample_rows: activation length %zu, in_dim %zu", in_dim, w->K);
     if (m == 0) return fail(c, SMX_ERR_ARG, "lm_head_sample_rows: zero rows");
+    if (w->N > SMX_SAMPLE_MAX_VOCAB) return fail(c, SMX_ERR_LIMIT, "lm_head_sample_rows: %zu tokens (%d)", w->N, SMX_SAMPLE_MAX_VOCAB);
     int rc;
     if ((rc = refuse_capture(c, "lm_head_sample_rows")) != SMX_OK) return rc;
     SMX_HIP(c, hipSetDevice(c->device));
@@ -420,7 +421,6 @@ int smx_lm_head_sample_rows(smx_ctx* c, const char* key, const float* xs, size_t
     }
     HostCall call(c);
     if ((rc = lm_head_logits(c, *w, xs, m)) != SMX_OK) return rc;
-    if (w->N > (size_t(1) << 22)) return fail(c, SMX_ERR_LIMIT, "lm_head_sample_rows: %zu tokens (2^22)", w->N);
     if ((rc = launch_sample(c, (const float*)c->yf32.p, m, w->N, w->N, &p, uu, ids, pr)) != SMX_OK) return rc;
     if ((rc = stream_wait(c)) != SMX_OK) return rc;
     memcpy(out, ids, m * 4);
