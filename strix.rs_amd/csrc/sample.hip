@@ -6,9 +6,9 @@
 //
 // Rows are ordered by (logit descending, index ascending), and nothing sorts a row.  Four launches over parts of rows:
 //   1  the largest logit
-//   2  rows with top_k or top_p: a histogram over kBins steps of distance from it, of tokens (top_k) or of weight (top_p)
-//   3  the bin that the cut falls into; what lies above it is totalled per chunk of kChunk tokens (top_k: listed), the bin's own
-//      tokens are listed
+//   2  rows with top_k or top_p: a histogram over kBins steps of distance from it, of tokens (top_k) or of weight (top_p), and in it
+//      the bin that the cut falls into
+//   3  what lies above the bin is totalled per chunk of kChunk tokens (top_k: listed), the bin's own tokens are listed
 //   4  one workgroup for each row sorts the list (up to kList tokens), which places the cut at one token, finds the chunk that
 //      the pick falls into from the totals and the pick in the chunk
 // A row is read three times (without top_k and top_p: twice), every other launch from its end, where the one in front has left
@@ -17,6 +17,7 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <type_traits>
 
 #include "smx_internal.h"
 
@@ -24,12 +25,14 @@ namespace smx {
 
 namespace {
 
-constexpr int kThreads = 1024, kWaves = kThreads / 64;   // of the row's own workgroup (launch 4)
+constexpr int kThreads = 256, kWaves = kThreads / 64;    // of the row's own workgroup (launch 4)
 constexpr int kChunk = 1024;                             // tokens whose kept weight is totalled together
-constexpr int kMaxVocab = SMX_SAMPLE_MAX_VOCAB, kMaxChunks = kMaxVocab / kChunk;
+constexpr int kMaxVocab = SMX_SAMPLE_MAX_VOCAB;   // (its chunks' totals are held in LDS)
 constexpr int kBins = 2048;
 constexpr float kReach = 28.0f;                          // exp(-28) < 2^-40: beyond it there is no weight
 constexpr int kList = 4096;
+constexpr int kSteps = 1024;                             // of a long list's keys
+constexpr int kWays = 7;                                 // keys that a step of the bisection tries
 
 struct SampleArgs {
     const float* logits;
@@ -40,11 +43,19 @@ struct SampleArgs {
     int* ids;
     float* prob;
     // workspace
-    uint2* best;                    // [rows][parts] key and index of the part's largest logit
+    unsigned long long* best;       // [rows][parts] candidate() of the part's largest logit
     unsigned long long* hist;       // [rows][kBins] weight; top_k rows: tokens
     unsigned long long* totals;     // [rows][chunks] kept weight above the cut's bin
     unsigned long long* list;       // [rows][kList] ~key : index
-    unsigned* listed;               // [rows]
+    struct RowCut* cuts;            // [rows]
+};
+
+// Where a row's cut is, found by the last workgroup of launch 2 to finish the row.
+struct RowCut {
+    unsigned long long above, limit;   // weight in front of the cut's bin; floor(top_p * all weight)   (top_p rows)
+    float total_from, list_from;       // logits from total_from on are kept, the ones below it from list_from on are the cut's bin
+    unsigned done;                     // workgroups of launch 2 that have added their part
+    unsigned listed;                   // tokens of the list
 };
 
 // Order-preserving key of a logit: NaN and -inf are 0, below every other; -0 is +0.
@@ -55,156 +66,229 @@ __device__ __forceinline__ unsigned key_of(float x) {
 }
 __device__ __forceinline__ float of_key(unsigned k) { return k == 0 ? -INFINITY : __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
-// exp((x - max) / T) of a candidate (x > -inf), 1 for the largest (so that a +inf maximum has a share)
-__device__ __forceinline__ float share(float x, float mx, float T) {
-#pragma clang fp contract(off)
-    return x == mx ? 1.0f : expf((x - mx) / T);
+// Division of distances by a row's temperature, correctly rounded, in three operations where the general one takes eleven: with
+// r = RN(1 / T), q = RN(a r) is within one unit of a / T, the remainder a - q T is exact in an FMA, and RN(q + remainder r) is the
+// correctly rounded quotient (Markstein's theorem, for divisors whose mantissa is not all ones).  Quotients below -200 keep q (their
+// exponential is 0); remainders lose bits to underflow only where |a / T| < 2^-40 (exponential 1).
+struct Temp {
+    float T, r;
+    bool quick;
+};
+__device__ __forceinline__ Temp temp_of(float T) {
+    const unsigned b = __float_as_uint(T);
+    return Temp{T, 1.0f / T, T > 0x1p-60f && T < 0x1p60f && (b & 0x7fffffu) != 0x7fffffu};
 }
-__device__ __forceinline__ unsigned long long weight(float e) { return (unsigned long long)(e * 0x1p40f); }
-// Bin of a candidate: steps of distance below the largest logit.  Rounding is monotone in x, so a smaller bin means a larger logit.
-__device__ __forceinline__ int bin_of(float x, float mx, float T) {
+__device__ __forceinline__ float over_T(float a, const Temp& t) {
 #pragma clang fp contract(off)
-    const float y = x == mx ? 0.0f : (mx - x) / T;
-    return (int)fminf(y * ((float)kBins / kReach), (float)(kBins - 1));
+    if (!t.quick) return a / t.T;   // (the same for the whole row)
+    const float q = a * t.r;
+    return q > -200.0f ? fmaf(fmaf(-q, t.T, a), t.r, q) : q;
 }
+// (x - max) / T of a candidate (x > -inf), 0 for the largest (so that a +inf maximum has a share)
+__device__ __forceinline__ float depth(float x, float mx, const Temp& t) {
+#pragma clang fp contract(off)
+    return x == mx ? 0.0f : over_T(x - mx, t);
+}
+// floor(e * 2^40) of an e in [0, 1], from its bits
+__device__ __forceinline__ unsigned long long weight(float e) {
+    const unsigned b = __float_as_uint(e);
+    return ((unsigned long long)((b & 0x7fffffu) | 0x800000u) << 17) >> min(127u - (b >> 23), 63u);
+}
+// Bin of a depth: steps of distance below the largest logit.  Every rounding is monotone in x, so a smaller bin means a larger logit.
+__device__ __forceinline__ int bin_of(float z) {
+#pragma clang fp contract(off)
+    return (int)fminf(z * -((float)kBins / kReach), (float)(kBins - 1));
+}
+
+// Steps over the lanes of a wave as DPP moves (a shuffle through LDS takes ten times as long, and launch 4 is a chain of them).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned long long dpp64(unsigned long long v) {   // 0 where no lane is moved from
+    const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)v, CTRL, ROWS, 0xf, false);
+    const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)(v >> 32), CTRL, ROWS, 0xf, false);
+    return (unsigned long long)hi << 32 | lo;
+}
+__device__ __forceinline__ unsigned long long wave_last(unsigned long long v) {   // lane 63's, in every lane
+    const unsigned lo = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)v, 63), hi = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)(v >> 32), 63);
+    return (unsigned long long)hi << 32 | lo;
+}
+__device__ __forceinline__ unsigned long long wave_scan(unsigned long long v) {   // inclusive sum
+    v += dpp64<0x111, 0xf>(v);   // row_shr 1, 2, 4, 8: sums inside each row of 16 lanes
+    v += dpp64<0x112, 0xf>(v);
+    v += dpp64<0x114, 0xf>(v);
+    v += dpp64<0x118, 0xf>(v);
+    v += dpp64<0x142, 0xa>(v);   // row_bcast 15 into rows 1 and 3, row_bcast 31 into rows 2 and 3
+    v += dpp64<0x143, 0xc>(v);
+    return v;
+}
+__device__ __forceinline__ unsigned long long wave_sum(unsigned long long v) { return wave_last(wave_scan(v)); }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned long long dpp_max(unsigned long long v) {
+    const unsigned long long o = dpp64<CTRL, ROWS>(v);
+    return o > v ? o : v;
+}
+__device__ __forceinline__ unsigned long long wave_max(unsigned long long v) {
+    v = dpp_max<0x111, 0xf>(v);
+    v = dpp_max<0x112, 0xf>(v);
+    v = dpp_max<0x114, 0xf>(v);
+    v = dpp_max<0x118, 0xf>(v);
+    v = dpp_max<0x142, 0xa>(v);
+    v = dpp_max<0x143, 0xc>(v);
+    return wave_last(v);
+}
+// A candidate for the largest logit: the larger word wins, on equal keys the lower index.
+__device__ __forceinline__ unsigned long long candidate(unsigned key, unsigned index) { return (unsigned long long)key << 32 | ~index; }
 
 // What a row asks for, and its largest logit.
 enum Mode { kNone, kGreedy, kFree, kTopK, kTopP };   // kNone: no candidate at all
 struct Ask {
     Mode mode;
     unsigned best_at;
-    float mx, T, top_p, min_p;
-    float bin_T;      // divides distances in bin_of: T, or 1 where tokens are counted
+    float mx, top_p, min_p;
+    Temp T, bin_T;    // bin_T divides distances for bin_of: T, or 1 where tokens are counted
     int top_k;
+    __device__ float share(float x) const { return expf(depth(x, mx, T)); }
+    __device__ int bin(float x) const { return bin_of(depth(x, mx, bin_T)); }
 };
-__device__ __forceinline__ uint2 better(uint2 a, uint2 b) { return b.x > a.x || (b.x == a.x && b.y < a.y) ? b : a; }
-__device__ __forceinline__ uint2 wave_best(uint2 v) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) v = better(v, make_uint2(__shfl_xor(v.x, o), __shfl_xor(v.y, o)));
-    return v;
-}
 __device__ __forceinline__ Ask ask_of(const SampleArgs& A, int row) {
     // every wave reads the parts' candidates for itself: no barrier
-    uint2 b = make_uint2(0u, 0xffffffffu);
-    for (int i = threadIdx.x & 63; i < A.parts; i += 64) b = better(b, A.best[(int64_t)row * A.parts + i]);
-    b = wave_best(b);
+    unsigned long long b = 0;
+    for (int i = threadIdx.x & 63; i < A.parts; i += 64) b = max(b, A.best[(int64_t)row * A.parts + i]);
+    b = wave_max(b);
+    const unsigned top = (unsigned)(b >> 32);
     Ask q;
-    q.best_at = b.y;
-    q.mx = of_key(b.x);
-    q.T = A.temperature ? A.temperature[row] : 1.0f;
+    q.best_at = ~(unsigned)b;
+    q.mx = of_key(top);
+    const float T = A.temperature ? A.temperature[row] : 1.0f;
+    q.T = temp_of(T);
     q.top_k = A.top_k ? A.top_k[row] : 0;
     q.top_p = A.top_p ? A.top_p[row] : 1.0f;
     q.min_p = A.min_p ? fminf(A.min_p[row], 1.0f) : 0.0f;
     const bool k = q.top_k > 0 && q.top_k < A.vocab;
-    q.mode = b.x == 0 ? kNone : !(q.T > 0.0f) || q.top_k == 1 || q.top_p <= 0.0f ? kGreedy : k ? kTopK : q.top_p < 1.0f ? kTopP : kFree;
-    q.bin_T = q.mode == kTopK ? 1.0f : q.T;
+    q.mode = top == 0 ? kNone : !(T > 0.0f) || q.top_k == 1 || q.top_p <= 0.0f ? kGreedy : k ? kTopK : q.top_p < 1.0f ? kTopP : kFree;
+    q.bin_T = q.mode == kTopK ? Temp{1.0f, 1.0f, true} : q.T;
     return q;
 }
 
-// The chunk's 16 tokens of each lane: token chunk * kChunk + 256 j + 4 lane + i (-inf past the row).
-template <bool VEC>
-__device__ __forceinline__ void load_chunk(const float* __restrict__ x, int vocab, int chunk, float (&v)[16]) {
-    const int lane = threadIdx.x & 63;
+// A row in chunks of kChunk tokens that start at 16-byte boundaries of memory: chunk c holds tokens kChunk c - skew ..., skew (0..3)
+// being how far the row's first token is behind such a boundary.
+struct Row {
+    const float* x;
+    int vocab, skew;
+};
+__device__ __forceinline__ Row row_of(const SampleArgs& A, int row) {
+    const float* x = A.logits + (int64_t)row * A.ld;
+    return Row{x, A.vocab, (int)((uintptr_t)x >> 2) & 3};
+}
+// A lane's 16 tokens of a chunk: token first_of + 256 j + i is v[4 j + i] (-inf outside the row).
+__device__ __forceinline__ int first_of(const Row& r, int chunk) { return chunk * kChunk - r.skew + 4 * (int)(threadIdx.x & 63); }
+__device__ __forceinline__ int token_of(int first, int n) { return first + 256 * (n >> 2) + (n & 3); }
+__device__ __forceinline__ void load_chunk(const Row& r, int chunk, float (&v)[16]) {
+    const int first = first_of(r, chunk);
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        const int i = chunk * kChunk + 256 * j + 4 * lane;
-        if (VEC && i + 4 <= vocab) {
-            const float4 f = *(const float4*)(x + i);
+        const int i = first + 256 * j;
+        if (i >= 0 && i + 4 <= r.vocab) {
+            const float4 f = *(const float4*)(r.x + i);
             v[4 * j] = f.x; v[4 * j + 1] = f.y; v[4 * j + 2] = f.z; v[4 * j + 3] = f.w;
         } else {
 #pragma unroll
-            for (int t = 0; t < 4; t++) v[4 * j + t] = i + t < vocab ? x[i + t] : -INFINITY;
+            for (int t = 0; t < 4; t++) v[4 * j + t] = i + t >= 0 && i + t < r.vocab ? r.x[i + t] : -INFINITY;
         }
     }
 }
-__device__ __forceinline__ int token_of(int chunk, int n) { return chunk * kChunk + 256 * (n >> 2) + 4 * (int)(threadIdx.x & 63) + (n & 3); }
 
 // Launch 1.  Workgroup (part, row); also clears what launches 2 and 3 add to.
-template <bool VEC>
 __global__ __launch_bounds__(1024) void sample_best_kernel(const SampleArgs A) {
-    __shared__ uint2 red[16];
+    __shared__ unsigned long long red[16];
     const int row = blockIdx.y, part = blockIdx.x, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-    const float* x = A.logits + (int64_t)row * A.ld;
+    const Row x = row_of(A, row);
     for (int i = part * blockDim.x + threadIdx.x; i < kBins; i += A.parts * blockDim.x) A.hist[(int64_t)row * kBins + i] = 0;
-    if (part == 0 && threadIdx.x == 0) A.listed[row] = 0;
-    uint2 b = make_uint2(0u, 0xffffffffu);
+    if (part == 0 && threadIdx.x == 0) { A.cuts[row].done = 0; A.cuts[row].listed = 0; }
+    unsigned bk = 0, bi = 0;
     const int c1 = min((part + 1) * A.part_chunks, A.chunks);
     for (int c = part * A.part_chunks + wave; c < c1; c += waves) {
         float v[16];
-        load_chunk<VEC>(x, A.vocab, c, v);
+        load_chunk(x, c, v);
+        const int first = first_of(x, c);
 #pragma unroll
-        for (int n = 0; n < 16; n++) {   // (ascending tokens of a lane: the first of equals stays)
+        for (int n = 0; n < 16; n++) {   // (a lane's tokens ascend: the first of equals stays)
             const unsigned k = key_of(v[n]);
-            if (k > b.x) b = make_uint2(k, (unsigned)token_of(c, n));
+            if (k > bk) { bk = k; bi = (unsigned)token_of(first, n); }
         }
     }
-    b = wave_best(b);
+    unsigned long long b = wave_max(candidate(bk, bi));
     if ((threadIdx.x & 63) == 0) red[wave] = b;
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int w = 1; w < waves; w++) b = better(b, red[w]);
+        for (int w = 1; w < waves; w++) b = max(b, red[w]);
         A.best[(int64_t)row * A.parts + part] = b;
     }
 }
 
-// Launch 2.  Workgroup (part, row), from the last to the first.
-template <bool VEC>
+// The smallest logit whose bin is below `bin` (comparing with it replaces a division for each token); NaN if there is none.
+// A wave tries 64 keys at a time.
+__device__ __forceinline__ float floor_of_bin(const Ask& q, int bin) {
+    const int lane = threadIdx.x & 63;
+    unsigned lo = key_of(-3.402823466e38f), hi = key_of(q.mx) + 1;   // none below lo; hi stands for none at all
+    const unsigned none = hi;
+    while (lo < hi) {
+        const unsigned step = (hi - lo + 63) / 64, k = min(lo + lane * step, hi);
+        const unsigned long long yes = __ballot(k == hi || q.bin(of_key(k)) < bin);
+        const int f = yes ? __ffsll((long long)yes) - 1 : 64;
+        const unsigned base = lo;
+        if (f > 0) lo = base + (f - 1) * step + 1;
+        if (f < 64) hi = min(base + f * step, hi);
+    }
+    return lo == none ? __uint_as_float(0x7fc00000u) : of_key(lo);
+}
+
+// Launch 2.  Workgroup (part, row), from the last to the first.  The last one of a row to finish reads the whole histogram: the
+// cut's bin is the first whose running total reaches top_k tokens, or floor(top_p * all weight).
 __global__ __launch_bounds__(1024) void sample_hist_kernel(const SampleArgs A) {
-    __shared__ unsigned long long hist[kBins];
+    __shared__ unsigned long long hist[kBins], red[16];
+    __shared__ unsigned done;
     const int row = A.rows - 1 - blockIdx.y, part = A.parts - 1 - blockIdx.x, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
     const Ask q = ask_of(A, row);
     if (q.mode != kTopK && q.mode != kTopP) return;
-    const float* x = A.logits + (int64_t)row * A.ld;
+    const Row x = row_of(A, row);
     for (int i = threadIdx.x; i < kBins; i += blockDim.x) hist[i] = 0;
     __syncthreads();
     const int c0 = part * A.part_chunks, c1 = min(c0 + A.part_chunks, A.chunks);
     for (int c = c1 - 1 - wave; c >= c0; c -= waves) {
         float v[16];
-        load_chunk<VEC>(x, A.vocab, c, v);
+        load_chunk(x, c, v);
 #pragma unroll
         for (int n = 0; n < 16; n++) {
             if (!(v[n] > -INFINITY)) continue;
-            const int b = bin_of(v[n], q.mx, q.bin_T);
-            const unsigned long long w = q.mode == kTopK ? 1ull : weight(share(v[n], q.mx, q.T));
-            if (w) atomicAdd(&hist[b], w);
+            const float z = depth(v[n], q.mx, q.bin_T);
+            const unsigned long long w = q.mode == kTopK ? 1ull : weight(expf(z));
+            if (w) atomicAdd(&hist[bin_of(z)], w);
         }
     }
     __syncthreads();
-    unsigned long long* out = A.hist + (int64_t)row * kBins;
+    unsigned long long* all = A.hist + (int64_t)row * kBins;
+    RowCut* cut = A.cuts + row;
     for (int i = threadIdx.x; i < kBins; i += blockDim.x) {
         const unsigned long long w = hist[i];
-        if (w) atomicAdd(&out[i], w);
+        if (w) atomicAdd(&all[i], w);
     }
-}
-
-__device__ __forceinline__ unsigned long long wave_sum(unsigned long long v) {
+    // What passes between workgroups is atomic at device scope, performed where all XCDs see it: this thread's additions are
+    // waited for, then the workgroup counts itself; the reads below are atomic too.  (A fence by each wave would write its XCD's L2
+    // back: 256 rows of 262144 329 us instead of 75.)
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0) done = atomicAdd(&cut->done, 1u);
+    __syncthreads();
+    if (done != (unsigned)A.parts - 1) return;
+    const int per = kBins / blockDim.x;   // neighbouring bins for each thread: 2..8
+    unsigned long long bins[8], sum = 0;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
-    return v;
-}
-__device__ __forceinline__ unsigned long long wave_scan(unsigned long long v) {   // inclusive
-    const int lane = threadIdx.x & 63;
+    for (int j = 0; j < 8; j++)   // (all in flight at once)
+        bins[j] = j < per ? __hip_atomic_load(&all[threadIdx.x * per + j], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const unsigned long long r = __shfl_up(v, o);
-        if (lane >= o) v += r;
-    }
-    return v;
-}
-
-// The cut's bin: the first whose running total reaches `limit` (top_k tokens, or floor(top_p * all weight)), and what lies above it.
-struct Cut {
-    int bin;
-    unsigned long long above, limit;
-};
-// Every thread of the workgroup (256..1024); red: 17 words of LDS.
-__device__ __forceinline__ Cut find_cut(const SampleArgs& A, const Ask& q, int row, unsigned long long* red) {
-    const unsigned long long* h = A.hist + (int64_t)row * kBins;
-    const int per = kBins / blockDim.x, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;   // bins of a thread: up to 8
-    unsigned long long mine[8], sum = 0;
-    for (int i = 0; i < per; i++) {
-        mine[i] = h[threadIdx.x * per + i];
-        sum += mine[i];
+    for (int j = 0; j < 8; j++) {
+        if (j < per) hist[threadIdx.x * per + j] = bins[j];
+        sum += bins[j];
     }
     unsigned long long run = wave_scan(sum);
     if ((threadIdx.x & 63) == 63) red[wave] = run;
@@ -215,69 +299,84 @@ __device__ __forceinline__ Cut find_cut(const SampleArgs& A, const Ask& q, int r
         total += red[w];
     }
     run += front - sum;   // in front of this thread's bins
-    Cut c;
-    c.limit = q.mode == kTopK ? (unsigned long long)q.top_k : (unsigned long long)((double)q.top_p * (double)total);
-    c.bin = kBins;        // fewer candidates than top_k: every one
-    c.above = 0;
+    const unsigned long long limit = q.mode == kTopK ? (unsigned long long)q.top_k : (unsigned long long)((double)q.top_p * (double)total);
+    // where the running total first reaches the limit; a limit of 0: the first bin; fewer candidates than top_k: behind the last bin
+    __shared__ int bin;
+    __shared__ unsigned long long above;
+    if (threadIdx.x == 0) { bin = limit == 0 ? 0 : kBins; above = limit == 0 ? 0 : total; }
     __syncthreads();
-    if (threadIdx.x == 0) { red[0] = kBins; red[1] = total; }
-    __syncthreads();
-    // the running total first reaches the limit in one thread's bins (a limit of 0: in the first bin)
-    if (run < c.limit && run + sum >= c.limit) {
-        for (int i = 0; i < per; i++) {
-            if (run + mine[i] >= c.limit) {
-                red[0] = threadIdx.x * per + i;
-                red[1] = run;
-                break;
-            }
-            run += mine[i];
-        }
+    if (run < limit && run + sum >= limit) {
+        int i = threadIdx.x * per;
+        while (run + hist[i] < limit) run += hist[i++];
+        bin = i;
+        above = run;
     }
-    if (c.limit == 0 && threadIdx.x == 0) { red[0] = 0; red[1] = 0; }
     __syncthreads();
-    c.bin = (int)red[0];
-    c.above = red[1];
-    return c;
+    if (wave < 2) {
+        const float f = floor_of_bin(q, bin + wave);
+        if ((threadIdx.x & 63) == 0) *(wave == 0 ? &cut->total_from : &cut->list_from) = wave == 0 && q.mode == kTopK ? __uint_as_float(0x7fc00000u) : f;
+    }
+    if (threadIdx.x == 0) { cut->above = above; cut->limit = limit; }
 }
 
 // Launch 3.  Workgroup (part, row).
-template <bool VEC>
 __global__ __launch_bounds__(1024) void sample_gather_kernel(const SampleArgs A) {
-    __shared__ unsigned long long red[17];
+    __shared__ unsigned long long list[kList];
+    __shared__ unsigned found, start;
     const int row = blockIdx.y, part = blockIdx.x, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, lane = threadIdx.x & 63;
     const Ask q = ask_of(A, row);
     if (q.mode <= kGreedy) return;
-    int cut = -1;
-    if (q.mode != kFree) cut = find_cut(A, q, row, red).bin;
-    const float* x = A.logits + (int64_t)row * A.ld;
+    if (threadIdx.x == 0) found = 0;
+    __syncthreads();
+    // (NaN: none; top_k rows list everything that they keep)
+    const float total_from = q.mode == kFree ? -3.402823466e38f : A.cuts[row].total_from;
+    const float list_from = q.mode == kFree ? __uint_as_float(0x7fc00000u) : A.cuts[row].list_from;
+    const Row x = row_of(A, row);
     const int c1 = min((part + 1) * A.part_chunks, A.chunks);
     for (int c = part * A.part_chunks + wave; c < c1; c += waves) {
         float v[16];
-        load_chunk<VEC>(x, A.vocab, c, v);
-        unsigned long long total = 0;
+        load_chunk(x, c, v);
+        const int first = first_of(x, c);
+        unsigned put = 0;
 #pragma unroll
-        for (int n = 0; n < 16; n++) {
-            const bool live = v[n] > -INFINITY;
-            const int b = q.mode != kFree ? bin_of(v[n], q.mx, q.bin_T) : -1;
-            if (live && q.mode != kTopK && (q.mode == kFree || b < cut)) {
-                const float e = share(v[n], q.mx, q.T);
-                if (e >= q.min_p) total += weight(e);
+        for (int n = 0; n < 16; n++) put |= (v[n] >= list_from && !(v[n] >= total_from) ? 1u : 0u) << n;
+        if (__ballot(put != 0)) {   // the wave's share of the workgroup's list: one LDS atomic for a chunk
+            const int mine = __popc(put);
+            int upto = mine;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int r = __shfl_up(upto, o);
+                if (lane >= o) upto += r;
             }
-            const bool put = live && (q.mode == kTopK ? b <= cut : q.mode == kTopP && b == cut);
-            const unsigned long long who = __ballot(put);
-            if (who) {
-                unsigned at = 0;
-                if (lane == 0) at = atomicAdd(&A.listed[row], (unsigned)__popcll(who));
-                at = __builtin_amdgcn_readfirstlane(at) + __popcll(who & ((1ull << lane) - 1));
-                if (put && at < (unsigned)kList)
-                    A.list[(int64_t)row * kList + at] = (unsigned long long)~key_of(v[n]) << 32 | (unsigned)token_of(c, n);
+            int at = 0;
+            if (lane == 63) at = (int)atomicAdd(&found, (unsigned)upto);
+            at = __shfl(at, 63) + upto - mine;
+            for (unsigned left = put; left; left &= left - 1, at++) {
+                if (at >= kList) break;
+                const int i = token_of(first, __ffs(left) - 1);
+                list[at] = (unsigned long long)~key_of(x.x[i]) << 32 | (unsigned)i;
             }
         }
         if (q.mode != kTopK) {
-            total = wave_sum(total);
+            double sum = 0;   // of 16 whole numbers up to 2^40: exact
+#pragma unroll
+            for (int n = 0; n < 16; n++) {
+                if (v[n] >= total_from) {
+                    const float e = q.share(v[n]);
+                    if (e >= q.min_p) sum += (double)truncf(e * 0x1p40f);
+                }
+            }
+            const unsigned long long total = wave_sum((unsigned long long)sum);
             if (lane == 0) A.totals[(int64_t)row * A.chunks + c] = total;
         }
     }
+    // behind the other parts' tokens in the row's list (what does not fit is only counted)
+    __syncthreads();
+    const unsigned n = found;
+    if (n == 0) return;
+    if (threadIdx.x == 0) start = atomicAdd(&A.cuts[row].listed, n);
+    __syncthreads();
+    for (unsigned i = threadIdx.x; i < n && start + i < (unsigned)kList; i += blockDim.x) A.list[(int64_t)row * kList + start + i] = list[i];
 }
 
 struct Reduce {
@@ -292,6 +391,15 @@ __device__ __forceinline__ unsigned long long block_sum(Reduce& r, unsigned long
     for (int w = 0; w < kWaves; w++) t += r.a[w];
     return t;
 }
+__device__ __forceinline__ unsigned long long block_max(Reduce& r, unsigned long long v) {
+    v = wave_max(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) r.a[threadIdx.x >> 6] = v;
+    __syncthreads();
+    unsigned long long t = 0;
+    for (int w = 0; w < kWaves; w++) t = max(t, r.a[w]);
+    return t;
+}
 // inclusive, over the workgroup's threads
 __device__ __forceinline__ unsigned long long block_scan(Reduce& r, unsigned long long v) {
     v = wave_scan(v);
@@ -302,21 +410,68 @@ __device__ __forceinline__ unsigned long long block_scan(Reduce& r, unsigned lon
     return v;
 }
 
-// Sorts a[0, n) upwards; n a power of two, up to kList.
-__device__ void sort_list(unsigned long long* a, int n) {
+// Sorts 2^m words upwards, word tid + kThreads e of them in v[e] of thread tid (bitonic; n <= kThreads E, the rest idle).  Steps of
+// less than a wave are exchanges between lanes, steps of kThreads and more are a thread's own, the ones between go through LDS.
+__device__ __forceinline__ unsigned long long lane_xor(unsigned long long v, int o) { return __shfl_xor(v, o); }
+template <int E>
+__device__ void sort_words(unsigned long long (&v)[E], unsigned long long* lds, int n) {
     for (int k = 2; k <= n; k <<= 1)
         for (int j = k >> 1; j > 0; j >>= 1) {
-            __syncthreads();
-            for (int t = threadIdx.x; t < n / 2; t += kThreads) {
-                const int i = ((t & ~(j - 1)) << 1) | (t & (j - 1));
-                const unsigned long long p = a[i], r = a[i | j];
-                const bool up = (i & k) == 0;
-                if ((p > r) == up) { a[i] = r; a[i | j] = p; }
+            if (j >= kThreads) {
+                const int ej = j / kThreads;
+#pragma unroll
+                for (int e = 0; e < E; e++)
+#pragma unroll
+                    for (int f = e + 1; f < E; f++)
+                        if (f == (e ^ ej)) {
+                            const bool up = ((e * kThreads) & k) == 0;
+                            const unsigned long long p = v[e], r = v[f];
+                            if ((p > r) == up) { v[e] = r; v[f] = p; }
+                        }
+            } else {
+                unsigned long long o[E];
+                if (j < 64) {
+#pragma unroll
+                    for (int e = 0; e < E; e++) o[e] = lane_xor(v[e], j);
+                } else {
+                    __syncthreads();
+#pragma unroll
+                    for (int e = 0; e < E; e++) lds[e * kThreads + threadIdx.x] = v[e];
+                    __syncthreads();
+#pragma unroll
+                    for (int e = 0; e < E; e++) o[e] = lds[e * kThreads + (threadIdx.x ^ j)];
+                }
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    const int i = e * kThreads + threadIdx.x;
+                    const bool up = (i & k) == 0, low = (i & j) == 0;
+                    v[e] = (v[e] < o[e]) == (up == low) ? v[e] : o[e];
+                }
             }
         }
     __syncthreads();
 }
-__device__ __forceinline__ int pow2_at_least(int n) { return n <= 1 ? 1 : 1 << (32 - __clz(n - 1)); }
+// The n words that from(i) gives, sorted upwards in a[0, n); n <= kList.
+template <class F>
+__device__ __forceinline__ void sort_list(unsigned long long* a, int n, F&& from) {
+    const int tid = threadIdx.x;
+    auto run = [&](auto tag, int size) {
+        constexpr int E = decltype(tag)::value;
+        unsigned long long v[E];
+#pragma unroll
+        for (int e = 0; e < E; e++) v[e] = e * kThreads + tid < n ? from(e * kThreads + tid) : ~0ull;
+        __syncthreads();   // `from` may have read a
+        sort_words<E>(v, a, size);
+#pragma unroll
+        for (int e = 0; e < E; e++) a[e * kThreads + tid] = v[e];
+        __syncthreads();
+    };
+    const int size = n <= 1 ? 1 : 1 << (32 - __clz(n - 1));
+    static_assert(kList <= 16 * kThreads, "16 words for each thread");
+    if (size <= kThreads) run(std::integral_constant<int, 1>{}, size);
+    else if (size <= 4 * kThreads) run(std::integral_constant<int, 4>{}, size);
+    else run(std::integral_constant<int, 16>{}, size);
+}
 
 // The last token that the cut keeps; tokens with a larger key, or its key and an index up to its own, are kept.
 struct Last {
@@ -324,23 +479,132 @@ struct Last {
 };
 __device__ __forceinline__ bool kept(const Last& l, unsigned k, unsigned i) { return k > l.key || (k == l.key && i <= l.at); }
 
+// The same for a list's word
+__device__ __forceinline__ bool kept(const Last& l, unsigned long long word) { return kept(l, ~(unsigned)(word >> 32), (unsigned)word); }
+__device__ __forceinline__ unsigned long long list_weight(const Ask& q, unsigned long long word) {
+    return weight(q.share(of_key(~(unsigned)(word >> 32))));
+}
+
+// Where the list's words that `bound` keeps, taken in order with `front` in front of them, reach `limit` (weight, or their number):
+// the last word with less than `limit` in front of it, at least the first one.  The words go into kSteps steps of their keys; the step
+// that the limit falls into is ordered by itself (thousands of equal logits: by index).
+__device__ Last place(const SampleArgs& A, const Ask& q, Reduce& red, const unsigned long long* list, int n, unsigned long long* step,
+                      unsigned long long* members, unsigned long long* found, Last bound, bool weighed, unsigned long long front, unsigned long long limit) {
+    const int tid = threadIdx.x;
+    unsigned lo = 0xffffffffu, hi = 0;
+    for (int i = tid; i < n; i += kThreads) {
+        lo = min(lo, (unsigned)(list[i] >> 32));
+        hi = max(hi, (unsigned)(list[i] >> 32));
+    }
+    lo = ~(unsigned)block_max(red, ~lo);
+    hi = (unsigned)block_max(red, hi);
+    const int shift = max(0, 22 - __clz(hi - lo | 1));   // (hi - lo) >> shift < kSteps
+    for (int i = tid; i < kSteps; i += kThreads) step[i] = 0;
+    if (tid == 0) { found[0] = kSteps; found[1] = 0; found[2] = 0; }
+    __syncthreads();
+    for (int i = tid; i < n; i += kThreads) {
+        const unsigned long long w = list[i];
+        if (kept(bound, w)) atomicAdd(&step[((unsigned)(w >> 32) - lo) >> shift], weighed ? list_weight(q, w) : 1ull);
+    }
+    __syncthreads();
+    constexpr int PER = kSteps / kThreads;
+    unsigned long long sum = 0;
+    for (int i = 0; i < PER; i++) sum += step[tid * PER + i];
+    unsigned long long run = front + block_scan(red, sum) - sum;
+    if (run < limit && run + sum >= limit) {
+        int i = tid * PER;
+        while (run + step[i] < limit) run += step[i++];
+        found[0] = i;
+        found[1] = run;
+    }
+    __syncthreads();
+    const unsigned at = limit <= front ? 0u : (unsigned)found[0];   // (nothing fits: the first word alone, which is in the first step)
+    if (at == kSteps) return bound;                                  // everything fits
+    run = limit <= front ? front : found[1];
+    for (int i = tid; i < n; i += kThreads) {
+        const unsigned long long w = list[i];
+        if (kept(bound, w) && ((unsigned)(w >> 32) - lo) >> shift == at) members[atomicAdd((unsigned*)&found[2], 1u)] = w;
+    }
+    __syncthreads();
+    const int m = (int)found[2];
+    unsigned long long mine = ~0ull, best = 0;
+    if (m <= kThreads) {
+        if (tid < m) mine = members[tid];
+        __syncthreads();
+        ulonglong2* const pairs = (ulonglong2*)members;
+        pairs[tid] = make_ulonglong2(mine, tid < m ? weighed ? list_weight(q, mine) : 1ull : 0ull);
+        __syncthreads();
+        bool first = true;
+#pragma unroll 8
+        for (int i = 0; i < m; i++) {
+            const ulonglong2 o = pairs[i];
+            const bool before = o.x < mine;
+            first = first && !before;
+            run += before ? o.y : 0;
+        }
+        if (tid < m && (first || run < limit)) best = mine;
+    } else {
+        sort_list(members, m, [&](int i) { return members[i]; });
+        const int per = (m + kThreads - 1) / kThreads, i0 = min(tid * per, m), i1 = min(i0 + per, m);
+        sum = 0;
+        for (int i = i0; i < i1; i++) sum += weighed ? list_weight(q, members[i]) : 1ull;
+        run += block_scan(red, sum) - sum;
+        for (int i = i0; i < i1; i++) {
+            if (i == 0 || run < limit) best = members[i];
+            run += weighed ? list_weight(q, members[i]) : 1ull;
+        }
+    }
+    best = block_max(red, best);
+    return Last{~(unsigned)(best >> 32), (unsigned)best};
+}
+
 // The cut of a row whose list overflowed, by bisection over the keys and then over the indices of the key's tokens.
 __device__ Last cut_by_bisection(const SampleArgs& A, const Ask& q, int row, Reduce& red) {
     const float* x = A.logits + (int64_t)row * A.ld;
     const int V = A.vocab;
-    // tokens and weight of keys > k
-    auto count_above = [&](unsigned k) {
-        unsigned long long t = 0;
-        for (int i = threadIdx.x; i < V; i += kThreads) t += key_of(x[i]) > k;
-        return block_sum(red, t);
-    };
-    auto weight_above = [&](unsigned k) {
-        unsigned long long t = 0;
+    // tokens, or weight, of keys > k for kWays keys k at once
+    auto above = [&](const unsigned (&k)[kWays], bool weighed, unsigned long long (&t)[kWays]) {
+#pragma unroll
+        for (int w = 0; w < kWays; w++) t[w] = 0;
         for (int i = threadIdx.x; i < V; i += kThreads) {
             const float v = x[i];
-            if (key_of(v) > k) t += weight(share(v, q.mx, q.T));
+            const unsigned key = key_of(v);
+            if (key <= k[0]) continue;
+            const unsigned long long m = weighed ? weight(q.share(v)) : 1ull;
+#pragma unroll
+            for (int w = 0; w < kWays; w++) t[w] += key > k[w] ? m : 0ull;
         }
-        return block_sum(red, t);
+#pragma unroll
+        for (int w = 0; w < kWays; w++) t[w] = block_sum(red, t[w]);
+    };
+    auto one_above = [&](unsigned k, bool weighed) {
+        unsigned ks[kWays];
+        unsigned long long t[kWays];
+#pragma unroll
+        for (int w = 0; w < kWays; w++) ks[w] = k;
+        above(ks, weighed, t);
+        return t[0];
+    };
+    // the smallest key in [lo, hi] with less than `limit` above it; hi has
+    auto smallest = [&](unsigned lo, unsigned hi, bool weighed, unsigned long long limit) {
+        while (lo < hi) {
+            const unsigned step = (hi - lo) / (kWays + 1) + 1;
+            unsigned ks[kWays];
+            unsigned long long t[kWays];
+#pragma unroll
+            for (int w = 0; w < kWays; w++) ks[w] = hi - lo > (unsigned)w * step ? lo + (unsigned)w * step : hi;
+            above(ks, weighed, t);
+            unsigned nlo = lo, nhi = hi;
+#pragma unroll
+            for (int w = kWays - 1; w >= 0; w--)
+                if (t[w] < limit) nhi = ks[w];
+#pragma unroll
+            for (int w = 0; w < kWays; w++)
+                if (!(t[w] < limit)) nlo = ks[w] + 1;
+            lo = nlo;
+            hi = nhi;
+        }
+        return lo;
     };
     // index of the n-th (from 1) token of key k, the last one if there are fewer
     auto nth = [&](unsigned k, unsigned long long n) {
@@ -357,28 +621,21 @@ __device__ Last cut_by_bisection(const SampleArgs& A, const Ask& q, int row, Red
     unsigned long long ties = 0;   // kept tokens of key l.key
     const unsigned top = key_of(q.mx);
     if (q.mode == kTopK) {
-        unsigned lo = 0, hi = top;
-        while (lo < hi) {          // the smallest key with fewer than top_k keys above it
-            const unsigned mid = lo + (hi - lo) / 2;
-            if (count_above(mid) < (unsigned long long)q.top_k) hi = mid; else lo = mid + 1;
-        }
+        unsigned lo = smallest(0u, top, false, (unsigned long long)q.top_k);   // fewer than top_k tokens above it
         if (lo == 0) lo = 1;       // (fewer candidates than top_k: all of them)
-        ties = min((unsigned long long)q.top_k - count_above(lo), count_above(lo - 1) - count_above(lo));
+        const unsigned long long front = one_above(lo, false);
+        ties = min((unsigned long long)q.top_k - front, one_above(lo - 1, false) - front);
         l.key = lo;
         l.at = ties ? nth(lo, ties) : 0u;
     }
     if (q.top_p < 1.0f) {
-        const unsigned long long w_key = l.key ? weight(share(of_key(l.key), q.mx, q.T)) : 0;
-        const unsigned long long total = weight_above(l.key) + ties * w_key;
+        const unsigned long long w_key = l.key ? weight(q.share(of_key(l.key))) : 0;
+        const unsigned long long total = one_above(l.key, true) + ties * w_key;
         const unsigned long long limit = (unsigned long long)((double)q.top_p * (double)total);
-        unsigned lo = l.key, hi = top;
-        while (lo < hi) {          // the smallest key with less than `limit` above it
-            const unsigned mid = lo + (hi - lo) / 2;
-            if (weight_above(mid) < limit) hi = mid; else lo = mid + 1;
-        }
         if (limit == 0) return Last{top, q.best_at};
-        const unsigned long long w = lo ? weight(share(of_key(lo), q.mx, q.T)) : 0;
-        const unsigned long long n = w ? (limit - weight_above(lo) + w - 1) / w : 0;
+        const unsigned lo = smallest(l.key, top, true, limit);
+        const unsigned long long w = lo ? weight(q.share(of_key(lo))) : 0;
+        const unsigned long long n = w ? (limit - one_above(lo, true) + w - 1) / w : 0;
         if (lo != l.key || n < ties) {
             l.key = lo;
             l.at = n ? nth(lo, n) : 0u;
@@ -390,11 +647,17 @@ __device__ Last cut_by_bisection(const SampleArgs& A, const Ask& q, int row, Red
 // Launch 4.  Workgroup: a row.
 __global__ __launch_bounds__(kThreads) void sample_pick_kernel(const SampleArgs A) {
     __shared__ Reduce red;
-    __shared__ unsigned long long list[kList];
-    __shared__ unsigned long long totals[kMaxChunks];
     __shared__ unsigned long long found[3];
+    extern __shared__ __align__(16) unsigned long long room[];   // list [kList], members [kList], totals [chunks] or steps [kSteps]
+    unsigned long long *const list = room, *const members = room + kList, *const totals = room + 2 * kList, *const step = totals;
+    unsigned long long* const ws = members;         // weights of a chunk
+    ulonglong2* const pairs = (ulonglong2*)members; // words and weights of a short list
+    const unsigned long long* sorted = list;
     const int row = blockIdx.x, tid = threadIdx.x;
-    const float* x = A.logits + (int64_t)row * A.ld;
+    const Row r = row_of(A, row);
+    const float* x = r.x;
+    const RowCut cut = A.cuts[row];   // (asked for with the row's parameters; means something where there is a cut)
+    const double u = A.u[row];
     const Ask q = ask_of(A, row);
     if (q.mode <= kGreedy) {
         if (tid == 0) {
@@ -403,154 +666,144 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(const SampleArgs 
         }
         return;
     }
-    const double u = A.u[row];
     Last last = {0u, 0xffffffffu};
-    int n = 0;
     bool fits = true;
-    Cut cut = {kBins, 0, 0};
+    int keep = 0;   // of the list, in order
     if (q.mode != kFree) {
-        cut = find_cut(A, q, row, list);
-        const unsigned listed = A.listed[row];
-        fits = listed <= (unsigned)kList;
-        if (fits) {
-            n = (int)listed;
-            const int size = pow2_at_least(n);
-            __syncthreads();
-            for (int i = tid; i < size; i += kThreads) list[i] = i < n ? A.list[(int64_t)row * kList + i] : ~0ull;
-            sort_list(list, size);
-        } else {
+        const unsigned long long* from = A.list + (int64_t)row * kList;
+        fits = cut.listed <= (unsigned)kList;
+        const int n = fits ? (int)cut.listed : 0;
+        if (!fits) {
             last = cut_by_bisection(A, q, row, red);
-        }
-    }
-    constexpr int PER = kList / kThreads;
-    unsigned long long w[PER];
-    if (fits && q.mode != kFree) {
-        // the list's tokens in order: thread t has PER of them
-        unsigned long long sum = 0;
-#pragma unroll
-        for (int j = 0; j < PER; j++) {
-            const int i = tid * PER + j;
-            w[j] = i < n && (q.mode != kTopK || i < q.top_k) ? weight(share(of_key(~(unsigned)(list[i] >> 32)), q.mx, q.T)) : 0;
-            sum += w[j];
-        }
-        unsigned long long ahead = block_scan(red, sum) - sum;
-        int keep = q.mode == kTopK ? min(n, q.top_k) : n;
-        if (q.top_p < 1.0f) {
-            unsigned long long limit = cut.limit;
-            if (q.mode == kTopK) {   // of what top_k has kept
-                const unsigned long long total = block_sum(red, sum);
-                limit = (unsigned long long)((double)q.top_p * (double)total);
-            } else {
-                ahead += cut.above;
-            }
-            unsigned long long c = 0;
-#pragma unroll
-            for (int j = 0; j < PER; j++) {
-                c += tid * PER + j < keep && ahead < limit;
-                ahead += w[j];
-            }
-            keep = max((int)block_sum(red, c), 1);
-        }
-        __syncthreads();
-        if (tid == 0) found[0] = keep;
-        if (q.mode == kTopK) {
-            // the pick in index order, among the list's first `keep`
-            const int size = pow2_at_least(keep);
-            unsigned long long mine[PER];
-#pragma unroll
-            for (int j = 0; j < PER; j++) {
-                const int i = tid + j * kThreads;
-                mine[j] = i < keep ? list[i] << 32 | list[i] >> 32 : ~0ull;   // index : ~key
-            }
+        } else if (n <= kThreads) {
+            // a token for each thread; its rank and the weight in front of it by comparing with every other
+            const unsigned long long mine = tid < n ? from[tid] : ~0ull;
+            const unsigned long long w = tid < n ? weight(q.share(of_key(~(unsigned)(mine >> 32)))) : 0;
+            list[tid] = mine;
+            pairs[tid] = make_ulonglong2(mine, w);
             __syncthreads();
-#pragma unroll
-            for (int j = 0; j < PER; j++)
-                if (tid + j * kThreads < size) list[tid + j * kThreads] = mine[j];
-            sort_list(list, size);
-            sum = 0;
-#pragma unroll
-            for (int j = 0; j < PER; j++) {
-                const int i = tid * PER + j;
-                w[j] = 0;
-                if (i < keep) {
-                    const float e = share(of_key(~(unsigned)list[i]), q.mx, q.T);
-                    if (e >= q.min_p) w[j] = weight(e);
-                }
-                sum += w[j];
+            int rank = 0;
+            unsigned long long ahead = 0;
+#pragma unroll 8
+            for (int i = 0; i < n; i++) {
+                const ulonglong2 o = pairs[i];
+                const bool before = o.x < mine;
+                rank += before;
+                ahead += before ? o.y : 0;
             }
-            const unsigned long long total = block_sum(red, sum);
-            const unsigned long long target = min((unsigned long long)fmax(u * (double)total, 0.0), total - 1);
-            unsigned long long run = block_scan(red, sum) - sum;
-#pragma unroll
-            for (int j = 0; j < PER; j++) {
-                if (run <= target && target < run + w[j]) {   // one token
-                    A.ids[row] = (int)(list[tid * PER + j] >> 32);
-                    if (A.prob) A.prob[row] = (float)((double)w[j] / (double)total);
-                }
-                run += w[j];
+            bool stay = tid < n && (q.mode != kTopK || rank < q.top_k);
+            if (q.top_p < 1.0f) {
+                unsigned long long limit = cut.limit;
+                if (q.mode == kTopK) limit = (unsigned long long)((double)q.top_p * (double)block_sum(red, stay ? w : 0));
+                else ahead += cut.above;
+                stay = stay && (rank == 0 || ahead < limit);
             }
-            return;
+            if (q.mode == kTopK) {
+                const float e = q.share(of_key(~(unsigned)(mine >> 32)));
+                const unsigned long long kw = stay && e >= q.min_p ? w : 0;
+                const unsigned long long total = block_sum(red, kw);
+                const unsigned long long target = min((unsigned long long)fmax(u * (double)total, 0.0), total - 1);
+                pairs[tid] = make_ulonglong2((unsigned)mine, kw);   // (read by everyone: block_sum has met since)
+                __syncthreads();
+                unsigned long long run = 0;   // kept weight of tokens in front of this one by index
+#pragma unroll 8
+                for (int i = 0; i < n; i++) {
+                    const ulonglong2 o = pairs[i];
+                    run += o.x < (unsigned)mine ? o.y : 0;
+                }
+                if (run <= target && target < run + kw) {
+                    A.ids[row] = (int)(unsigned)mine;
+                    if (A.prob) A.prob[row] = (float)((double)kw / (double)total);
+                }
+                return;
+            }
+            const int count = (int)block_sum(red, stay);
+            if (stay && rank == count - 1) found[0] = mine;
+            __syncthreads();
+            last = Last{~(unsigned)(found[0] >> 32), (unsigned)found[0]};
+            keep = n;
+        } else {
+            for (int i = tid; i < n; i += kThreads) list[i] = from[i];
+            __syncthreads();
+            // (a cut in LDS: the list by kSteps steps of its keys, then the step's own tokens)
+            if (q.mode == kTopK) {
+                last = place(A, q, red, list, n, step, members, found, last, false, 0, (unsigned long long)q.top_k);
+                if (q.top_p < 1.0f) {
+                    unsigned long long t = 0;
+                    for (int i = tid; i < n; i += kThreads) t += kept(last, list[i]) ? list_weight(q, list[i]) : 0;
+                    const unsigned long long limit = (unsigned long long)((double)q.top_p * (double)block_sum(red, t));   // of what top_k has kept
+                    last = place(A, q, red, list, n, step, members, found, last, true, 0, limit);
+                }
+            } else {
+                last = place(A, q, red, list, n, step, members, found, last, true, cut.above, cut.limit);
+            }
+            keep = n;
+            sorted = list;
         }
-        last = Last{~(unsigned)(list[keep - 1] >> 32), (unsigned)list[keep - 1]};
     }
     // the chunks' totals
-    for (int c = tid; c < A.chunks; c += kThreads) totals[c] = fits ? A.totals[(int64_t)row * A.chunks + c] : 0;
+    for (int c = tid; c < A.chunks; c += kThreads) totals[c] = fits && q.mode != kTopK ? A.totals[(int64_t)row * A.chunks + c] : 0;
     __syncthreads();
     if (!fits) {
         for (int c = tid >> 6; c < A.chunks; c += kWaves) {
             unsigned long long t = 0;
-            for (int i = c * kChunk + (tid & 63); i < min((c + 1) * kChunk, A.vocab); i += 64) {
+            for (int i = max(c * kChunk - r.skew, 0) + (tid & 63); i < min((c + 1) * kChunk - r.skew, A.vocab); i += 64) {
                 const float v = x[i];
                 if (v > -INFINITY && kept(last, key_of(v), (unsigned)i)) {
-                    const float e = share(v, q.mx, q.T);
+                    const float e = q.share(v);
                     if (e >= q.min_p) t += weight(e);
                 }
             }
             t = wave_sum(t);
             if ((tid & 63) == 0) totals[c] = t;
         }
-    } else if (q.mode == kTopP) {
-        const int keep = (int)found[0];
-        for (int i = tid; i < keep; i += kThreads) {
-            const float e = share(of_key(~(unsigned)(list[i] >> 32)), q.mx, q.T);
-            if (e >= q.min_p) atomicAdd(&totals[(unsigned)list[i] / kChunk], weight(e));
+    } else {
+        for (int i = tid; i < keep; i += kThreads) {   // the list's kept tokens (none without a cut)
+            const float e = q.share(of_key(~(unsigned)(sorted[i] >> 32)));
+            if (kept(last, sorted[i]) && e >= q.min_p) atomicAdd(&totals[((unsigned)sorted[i] + r.skew) / kChunk], weight(e));
         }
     }
     __syncthreads();
-    constexpr int CPT = kMaxChunks / kThreads;
-    unsigned long long t[CPT], sum = 0;
-#pragma unroll
-    for (int j = 0; j < CPT; j++) {
-        const int c = tid * CPT + j;
-        t[j] = c < A.chunks ? totals[c] : 0;
-        sum += t[j];
-    }
-    unsigned long long run = block_scan(red, sum);
-    if (tid == kThreads - 1) found[0] = run;
-    __syncthreads();
-    const unsigned long long total = found[0];
+    const int per = (A.chunks + kThreads - 1) / kThreads, c0 = min(tid * per, A.chunks), c1 = min(c0 + per, A.chunks);
+    unsigned long long sum = 0;
+    for (int c = c0; c < c1; c++) sum += totals[c];
+    const unsigned long long total = block_sum(red, sum);
     const unsigned long long target = min((unsigned long long)fmax(u * (double)total, 0.0), total - 1);
-    run -= sum;
-#pragma unroll
-    for (int j = 0; j < CPT; j++) {
-        if (run <= target && target < run + t[j]) { found[1] = tid * CPT + j; found[2] = target - run; }
-        run += t[j];
+    unsigned long long run = block_scan(red, sum) - sum;
+    if (run <= target && target < run + sum) {
+        int c = c0;
+        while (run + totals[c] <= target) run += totals[c++];
+        found[0] = c;
+        found[1] = target - run;
     }
     __syncthreads();
-    // the pick in its chunk: one token for each thread
-    static_assert(kChunk == kThreads, "a token for each thread");
-    const unsigned i = (unsigned)found[1] * kChunk + tid;
-    const unsigned long long left = found[2];
-    const float v = i < (unsigned)A.vocab ? x[i] : -INFINITY;
-    unsigned long long mine = 0;
-    if (v > -INFINITY && kept(last, key_of(v), i)) {
-        const float e = share(v, q.mx, q.T);
-        if (e >= q.min_p) mine = weight(e);
+    // the pick in its chunk: neighbouring tokens for each thread
+    constexpr int PICK = kChunk / kThreads;
+    const int first = (int)found[0] * kChunk + tid * PICK - r.skew;
+    const unsigned long long left = found[1];
+    float v[PICK];
+#pragma unroll
+    for (int j = 0; j < PICK; j++) v[j] = first + j >= 0 && first + j < A.vocab ? x[first + j] : -INFINITY;
+    float* const vs = (float*)list;
+#pragma unroll
+    for (int j = 0; j < PICK; j++) vs[tid * PICK + j] = v[j];   // (a thread's own: a rolled loop over registers)
+    sum = 0;
+#pragma unroll 1
+    for (int j = tid * PICK; j < tid * PICK + PICK; j++) {
+        unsigned long long w = 0;
+        if (vs[j] > -INFINITY && kept(last, key_of(vs[j]), (unsigned)(first + j - tid * PICK))) {
+            const float e = q.share(vs[j]);
+            if (e >= q.min_p) w = weight(e);
+        }
+        ws[j] = w;
+        sum += w;
     }
-    const unsigned long long upto = block_scan(red, mine);
-    if (upto - mine <= left && left < upto) {
-        A.ids[row] = (int)i;
-        if (A.prob) A.prob[row] = (float)((double)mine / (double)total);
+    run = block_scan(red, sum) - sum;
+    if (run <= left && left < run + sum) {
+        int j = tid * PICK;
+        while (run + ws[j] <= left) run += ws[j++];
+        A.ids[row] = first + j - tid * PICK;
+        if (A.prob) A.prob[row] = (float)((double)ws[j] / (double)total);
     }
 }
 
@@ -559,7 +812,7 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(const SampleArgs 
 int launch_sample(smx_ctx* c, const float* logits, size_t rows, size_t vocab, size_t ld, const smx_sample_params* p, const float* u, int32_t* ids, float* prob) {
     SampleArgs A{};
     A.logits = logits; A.ld = (int64_t)ld; A.rows = (int)rows; A.vocab = (int)vocab;
-    A.chunks = (int)((vocab + kChunk - 1) / kChunk);
+    A.chunks = (int)((vocab + 3 + kChunk - 1) / kChunk);   // (a row may start up to 3 tokens into its first chunk)
     if (p) { A.temperature = p->temperature; A.top_k = p->top_k; A.top_p = p->top_p; A.min_p = p->min_p; }
     A.u = u; A.ids = ids; A.prob = prob;
     // Parts of a row: 512 workgroups in all (two a CU), of at least one chunk a wave.  Few rows take workgroups of 4 waves, so that
@@ -573,17 +826,18 @@ int launch_sample(smx_ctx* c, const float* logits, size_t rows, size_t vocab, si
     // workspace of up to kRowsAtOnce rows (the launches of a larger call follow one another)
     constexpr size_t kRowsAtOnce = 4096;
     const size_t group = std::min(rows, kRowsAtOnce);
-    const size_t per_row = (size_t)kBins * 8 + (size_t)A.chunks * 8 + (size_t)kList * 8 + (size_t)A.parts * 8 + 4;
+    const size_t per_row = (size_t)kBins * 8 + (size_t)A.chunks * 8 + (size_t)kList * 8 + (size_t)A.parts * 8 + sizeof(RowCut);
     int rc;
     if ((rc = ensure(c, c->work, group * per_row + 64)) != SMX_OK) return rc;
     A.hist = (unsigned long long*)c->work.p;
     A.totals = A.hist + group * kBins;
     A.list = A.totals + group * A.chunks;
-    A.best = (uint2*)(A.list + group * kList);
-    A.listed = (unsigned*)(A.best + group * A.parts);
-    const bool vec = ld % 4 == 0 && ((uintptr_t)logits & 15) == 0;
+    A.best = A.list + group * kList;
+    A.cuts = (RowCut*)(A.best + group * A.parts);
     // Without top_k and top_p arrays no row has a cut: no histogram.
     const bool cuts = A.top_k || A.top_p;
+    const size_t lds = (2 * (size_t)kList + std::max(A.chunks, kSteps)) * 8;
+    if ((rc = set_dyn_lds(c, sample_pick_kernel, lds)) != SMX_OK) return rc;
     ProfScope ps(c, "sample");
     for (size_t r = 0; r < rows; r += group) {
         SampleArgs G = A;
@@ -597,10 +851,10 @@ int launch_sample(smx_ctx* c, const float* logits, size_t rows, size_t vocab, si
         G.u += r; G.ids += r;
         if (prob) G.prob += r;
         const dim3 grid((unsigned)A.parts, (unsigned)n);
-        hipLaunchKernelGGL(vec ? sample_best_kernel<true> : sample_best_kernel<false>, grid, dim3(threads), 0, c->stream, G);
-        if (cuts) hipLaunchKernelGGL(vec ? sample_hist_kernel<true> : sample_hist_kernel<false>, grid, dim3(threads), 0, c->stream, G);
-        hipLaunchKernelGGL(vec ? sample_gather_kernel<true> : sample_gather_kernel<false>, grid, dim3(threads), 0, c->stream, G);
-        hipLaunchKernelGGL(sample_pick_kernel, dim3((unsigned)n), dim3(kThreads), 0, c->stream, G);
+        hipLaunchKernelGGL(sample_best_kernel, grid, dim3(threads), 0, c->stream, G);
+        if (cuts) hipLaunchKernelGGL(sample_hist_kernel, grid, dim3(threads), 0, c->stream, G);
+        hipLaunchKernelGGL(sample_gather_kernel, grid, dim3(threads), 0, c->stream, G);
+        hipLaunchKernelGGL(sample_pick_kernel, dim3((unsigned)n), dim3(kThreads), lds, c->stream, G);
         SMX_HIP(c, hipGetLastError());
     }
     return SMX_OK;

@@ -202,3 +202,33 @@ def test_refusals(accel, pkg):
                 accel.sample_dev(*a)
         with pytest.raises(pkg.SmxError):
             accel.sample_dev(p, 2, 100, p, p, ld=99)
+
+
+@pytest.mark.parametrize("v", [700, 9000, 40000])
+@pytest.mark.parametrize("levels", [1, 3, 400])
+def test_many_equal_logits(accel, v, levels):
+    """Logits of a few levels (as bf16 logits of a large vocabulary are): cuts inside thousands of equal tokens, by index."""
+    rng = np.random.default_rng(v + levels)
+    rows = 16
+    x = (rng.integers(0, levels, (rows, v)) * (6.0 / max(1, levels - 1))).astype(np.float32)
+    u = rng.random(rows, dtype=np.float32)
+    k = np.array([0, 0, 0, 0, 2, 100, 255, 256, 257, 600, 3000, 4096, 4097, 8000, v - 1, v], np.int32)
+    p = np.array([0.05, 0.5, 0.95, 1, 1, 0.5, 0.9, 1, 0.3, 0.7, 1, 0.6, 1, 0.8, 1, 0.2], np.float32)
+    T = np.where(np.arange(rows) % 2 == 0, 1.0, 2.5).astype(np.float32)
+    m = np.where(np.arange(rows) % 5 == 3, 0.01, 0.0).astype(np.float32)
+    ids, prob = _run(accel, x, u, T, k, p, m, gap=v % 3)
+    _check(x, ids, prob, u, T, k, p, m)
+
+
+def test_cut_far_below_the_largest(accel):
+    """top_k reaches past a gap of hundreds between logits."""
+    rng = np.random.default_rng(8)
+    v = 6000
+    x = rng.standard_normal((4, v)).astype(np.float32)
+    x[:, 17] = 300
+    x[2:, 40:] -= 1000
+    k = np.array([50, 5000, 30, 4500], np.int32)
+    T = np.full(4, 100.0, np.float32)
+    u = np.array([0.3, 0.99, 0.6, 0.9], np.float32)
+    ids, prob = _run(accel, x, u, T, k)
+    _check(x, ids, prob, u, T, k, None, None)
