@@ -812,7 +812,9 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(const SampleArgs 
 int launch_sample(smx_ctx* c, const float* logits, size_t rows, size_t vocab, size_t ld, const smx_sample_params* p, const float* u, int32_t* ids, float* prob) {
     SampleArgs A{};
     A.logits = logits; A.ld = (int64_t)ld; A.rows = (int)rows; A.vocab = (int)vocab;
-    A.chunks = (int)((vocab + 3 + kChunk - 1) / kChunk);   // (a row may start up to 3 tokens into its first chunk)
+// (rows that do not all start at 16-byte boundaries may lie up to 3 tokens into their first chunk)
+    const size_t skew = ld % 4 == 0 ? ((uintptr_t)logits >> 2) & 3 : 3;
+    A.chunks = (int)((vocab + skew + kChunk - 1) / kChunk);
     if (p) { A.temperature = p->temperature; A.top_k = p->top_k; A.top_p = p->top_p; A.min_p = p->min_p; }
     A.u = u; A.ids = ids; A.prob = prob;
     // Parts of a row: 512 workgroups in all (two a CU), of at least one chunk a wave.  Few rows take workgroups of 4 waves, so that
@@ -821,7 +823,8 @@ int launch_sample(smx_ctx* c, const float* logits, size_t rows, size_t vocab, si
     const int threads = few ? 256 : 1024;
     const size_t want = 512, most = ((size_t)A.chunks + threads / 64 - 1) / (threads / 64);
     size_t parts = std::max<size_t>(1, std::min(most, (want + rows - 1) / rows));
-    A.part_chunks = (int)((A.chunks + parts - 1) / parts);
+    const size_t waves = threads / 64;   // whole rounds of the waves
+    A.part_chunks = (int)std::max<size_t>(waves, ((A.chunks + parts - 1) / parts + waves / 2) / waves * waves);
     A.parts = (A.chunks + A.part_chunks - 1) / A.part_chunks;
     // workspace of up to kRowsAtOnce rows (the launches of a larger call follow one another)
     constexpr size_t kRowsAtOnce = 4096;
