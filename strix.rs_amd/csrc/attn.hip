@@ -31,6 +31,7 @@ typedef float v4f __attribute__((ext_vector_type(4)));
 constexpr int kSegBlocks = 128;          // blocks whose places and scales are looked up at a time
 constexpr float kLazy = 8.0f;            // the running maximum follows only steps of more than 2^8
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kMaxPieces = 1024;
 constexpr float kNoMax = -1e30f;         // running maximum of a row that has seen no key
 
 struct AttnArgs {
@@ -76,6 +77,12 @@ __device__ __forceinline__ v8h widen8(unsigned lo, unsigned hi) {
     widen4(lo, p);
     widen4(hi, p + 2);
     return __builtin_bit_cast(v8h, r);
+}
+
+// A value that is the same in every lane of a wave, in scalar registers.
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+    const unsigned lo = __builtin_amdgcn_readfirstlane((int)(unsigned)v), hi = __builtin_amdgcn_readfirstlane((int)(unsigned)((uint64_t)v >> 32));
+    return (int64_t)((uint64_t)hi << 32 | lo);
 }
 
 // Largest of the four lanes that share a row (lane, lane ^ 16, lane ^ 32, lane ^ 48), and their sum.
@@ -248,7 +255,7 @@ __device__ __forceinline__ void put_row(const AttnArgs& A, const RowAt& r, int p
 // sequence); its four waves take the piece's blocks in turn, straight from memory into the matrix instructions' registers (one block
 // ahead), and add up through LDS at the end.
 template <int DC, int CT, int NT, bool BF16>
-__global__ __launch_bounds__(256) void attn_rows_kernel(const AttnArgs A) {
+__global__ __launch_bounds__(256, CT == 2 ? 2 : DC <= 1 ? 4 : DC == 2 ? 3 : 2) void attn_rows_kernel(const AttnArgs A) {
     constexpr int D64 = DC * 64, NO = DC * 4;
     __shared__ Segment seg;
     __shared__ float wm[4][16 * CT], wl[4][16 * CT];
@@ -302,52 +309,51 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(const AttnArgs A) {
             vexp = e;
         }
         const float vup = pow2(vexp);
+        // a block's bytes are asked for as soon as the registers of the one in front are free: keys behind its scores, values behind
+        // its second product
         uint4 kb[2 * DC], vb[2 * DC];
-        auto fetch = [&](int i) {
-            const int64_t base = seg.place[i] * (SMX_KV_BLOCK * D64) + lane * 16;
+        auto fetch = [&](uint4 (&to)[2 * DC], const int8_t* plane, int i) {
+            const int8_t* base = plane + uniform(seg.place[i]) * (SMX_KV_BLOCK * D64);
 #pragma unroll
-            for (int j = 0; j < 2 * DC; j++) kb[j] = *(const uint4*)(A.kv.k + base + j * 1024);
-#pragma unroll
-            for (int j = 0; j < 2 * DC; j++) vb[j] = *(const uint4*)(A.kv.v + base + j * 1024);
+            for (int j = 0; j < 2 * DC; j++) to[j] = *(const uint4*)(base + (unsigned)(j * 1024 + lane * 16));
         };
-        if (wave < n) fetch(wave);
+        if (wave < n) {
+            fetch(kb, A.kv.k, wave);
+            fetch(vb, A.kv.v, wave);
+        }
         for (int i = wave; i < n; i += 4) {
-            v8h kf[2][DC * 2];
+            v4f sc[CT][2];
 #pragma unroll
-            for (int tt = 0; tt < 2; tt++)
+            for (int tt = 0; tt < 2; tt++) {
+                v8h kf[DC * 2];
 #pragma unroll
                 for (int c = 0; c < DC; c++) {
                     const uint4 w = kb[tt * DC + c];
-                    kf[tt][c * 2] = widen8(w.x, w.y);
-                    kf[tt][c * 2 + 1] = widen8(w.z, w.w);
+                    kf[c * 2] = widen8(w.x, w.y);
+                    kf[c * 2 + 1] = widen8(w.z, w.w);
                 }
-            v8h vf[NO];
 #pragma unroll
-            for (int j = 0; j < 2 * DC; j++) {
-                vf[2 * j] = widen8(vb[j].x, vb[j].y);
-                vf[2 * j + 1] = widen8(vb[j].z, vb[j].w);
+                for (int ct = 0; ct < CT; ct++) {
+                    sc[ct][tt] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int nt = NT - 1; nt >= 0; nt--)   // the small terms first: fewer roundings of large sums
+#pragma unroll
+                        for (int k = 0; k < DC * 2; k++) sc[ct][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[k], qf[ct][nt][k], sc[ct][tt], 0, 0, 0);
+                }
             }
             const float ks = seg.ks[i], vs = seg.vs[i] * vup;
-            if (i + 4 < n) fetch(i + 4);
+            const int next = i + 4;
+            if (next < n) fetch(kb, A.kv.k, next);
             const int tok = (c0 + i) * SMX_KV_BLOCK;
             const bool edge = tok + SMX_KV_BLOCK - 1 > all_hi || tok < all_lo;
             float t[CT][8], mx[CT];
 #pragma unroll
             for (int ct = 0; ct < CT; ct++) {
-                v4f sc[2];
-#pragma unroll
-                for (int tt = 0; tt < 2; tt++) {
-                    sc[tt] = v4f{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int k = 0; k < DC * 2; k++)
-#pragma unroll
-                        for (int nt = 0; nt < NT; nt++) sc[tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[tt][k], qf[ct][nt][k], sc[tt], 0, 0, 0);
-                }
                 const float f = unit[ct] * ks;
                 mx[ct] = kNoMax;
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    t[ct][j] = sc[j >> 2][j & 3] * f;
+                    t[ct][j] = sc[ct][j >> 2][j & 3] * f;
                     if (edge) {
                         const int key = tok + 16 * (j >> 2) + 4 * g + (j & 3);
                         if (key > at[ct].pos || (A.window > 0 && key <= at[ct].pos - A.window)) t[ct][j] = -INFINITY;
@@ -357,22 +363,31 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(const AttnArgs A) {
                 mx[ct] = row_max(mx[ct]);
             }
             rescale<CT, NO>(mx, m, l, o);
+            v8h pf[CT][NT];
 #pragma unroll
             for (int ct = 0; ct < CT; ct++) {
-                float p[8];
+                float p[8], sum = 0.f;
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     const float e2 = __builtin_amdgcn_exp2f(t[ct][j] - m[ct]);
-                    l[ct] += e2;
+                    sum += e2;
                     p[j] = edge && t[ct][j] == -INFINITY ? 0.f : e2 * vs;   // (a masked token's value scale may be NaN)
                 }
-                v8h pf[NT];
-                split_prob<NT>(p, pf);
-#pragma unroll
-                for (int k = 0; k < NO; k++)
-#pragma unroll
-                    for (int nt = 0; nt < NT; nt++) o[ct][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[k], pf[nt], o[ct][k], 0, 0, 0);
+                l[ct] += sum;
+                split_prob<NT>(p, pf[ct]);
             }
+#pragma unroll
+            for (int j = 0; j < 2 * DC; j++) {
+                const v8h v0 = widen8(vb[j].x, vb[j].y), v1 = widen8(vb[j].z, vb[j].w);
+#pragma unroll
+                for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+                    for (int nt = NT - 1; nt >= 0; nt--) {
+                        o[ct][2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pf[ct][nt], o[ct][2 * j], 0, 0, 0);
+                        o[ct][2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pf[ct][nt], o[ct][2 * j + 1], 0, 0, 0);
+                    }
+            }
+            if (next < n) fetch(vb, A.kv.v, next);
         }
     }
     // the four waves' shares
@@ -414,7 +429,7 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(const AttnArgs A) {
 // share tiles of 64 tokens that are widened to f16 on their way into LDS (each byte once per workgroup).  The next tile's bytes are
 // in flight while one is computed.
 template <int DC, int CT, int NT, bool BF16>
-__global__ __launch_bounds__(256) void attn_tile_kernel(const AttnArgs A) {
+__global__ __launch_bounds__(256, 2) void attn_tile_kernel(const AttnArgs A) {
     constexpr int D64 = DC * 64, NO = DC * 4, KF = DC * 2;
     __shared__ Segment seg;
     extern __shared__ uint4 stage[];   // keys [4 token tiles][KF][64 lanes], values [2 blocks][NO][64 lanes], 8 f16 each
@@ -506,14 +521,15 @@ __global__ __launch_bounds__(256) void attn_tile_kernel(const AttnArgs A) {
             for (int tt = 0; tt < 4; tt++) {
 #pragma unroll
                 for (int ct = 0; ct < CT; ct++) sc[ct][tt] = v4f{0.f, 0.f, 0.f, 0.f};
+                v8h kf[KF];
 #pragma unroll
-                for (int k = 0; k < KF; k++) {
-                    const v8h kf = __builtin_bit_cast(v8h, kt[(tt * KF + k) * 64 + lane]);
+                for (int k = 0; k < KF; k++) kf[k] = __builtin_bit_cast(v8h, kt[(tt * KF + k) * 64 + lane]);
 #pragma unroll
-                    for (int ct = 0; ct < CT; ct++)
+                for (int nt = NT - 1; nt >= 0; nt--)   // the small terms first: fewer roundings of large sums
 #pragma unroll
-                        for (int nt = 0; nt < NT; nt++) sc[ct][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[ct][nt][k], sc[ct][tt], 0, 0, 0);
-                }
+                    for (int k = 0; k < KF; k++)
+#pragma unroll
+                        for (int ct = 0; ct < CT; ct++) sc[ct][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[k], qf[ct][nt][k], sc[ct][tt], 0, 0, 0);
             }
             float mx[CT];
 #pragma unroll
@@ -540,14 +556,15 @@ __global__ __launch_bounds__(256) void attn_tile_kernel(const AttnArgs A) {
                 v8h pf[CT][NT];
 #pragma unroll
                 for (int ct = 0; ct < CT; ct++) {
-                    float p[8];
+                    float p[8], sum = 0.f;
 #pragma unroll
                     for (int j = 0; j < 8; j++) {
                         const float t = sc[ct][2 * b + (j >> 2)][j & 3];
                         const float e2 = __builtin_amdgcn_exp2f(t - m[ct]);
-                        l[ct] += e2;
+                        sum += e2;
                         p[j] = edge && t == -INFINITY ? 0.f : e2 * vs[b];
                     }
+                    l[ct] += sum;
                     split_prob<NT>(p, pf[ct]);
                 }
 #pragma unroll
@@ -556,7 +573,7 @@ __global__ __launch_bounds__(256) void attn_tile_kernel(const AttnArgs A) {
 #pragma unroll
                     for (int ct = 0; ct < CT; ct++)
 #pragma unroll
-                        for (int nt = 0; nt < NT; nt++) o[ct][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[ct][nt], o[ct][k], 0, 0, 0);
+                        for (int nt = NT - 1; nt >= 0; nt--) o[ct][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[ct][nt], o[ct][k], 0, 0, 0);
                 }
             }
         }
@@ -570,11 +587,13 @@ __global__ __launch_bounds__(256) void attn_tile_kernel(const AttnArgs A) {
     }
 }
 
-// Workgroup (row, head): the pieces of a long sequence joined.  Thread group w of 4 adds up every fourth piece.
+// Workgroup (row, head): the pieces of a long sequence joined.  Every piece's factor is formed first, so that nothing stands between
+// the loads of their sums; 16 bytes for each thread, several pieces at a time.
 template <bool BF16>
 __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs A) {
-    __shared__ float sums[4][SMX_KV_MAX_HEAD_DIM], red[4];
-    const int row = blockIdx.x, head = blockIdx.y;
+    __shared__ float factor[kMaxPieces], red[2][4];
+    __shared__ v4f sums[256];
+    const int row = blockIdx.x, head = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int s = row;
     if (A.kv.row0) {
         int lo = 0, hi = A.kv.nseq - 1;
@@ -586,30 +605,37 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs A) {
     }
     const Span sp = seq_span(A, s);
     if (sp.pieces <= 1 || row >= sp.q.row + sp.q.n) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t at = ((int64_t)row * A.q_heads + head) * A.pieces;
     float M = kNoMax;
-    for (int i = lane; i < sp.pieces; i += 64) M = fmaxf(M, A.part_ml[at + i].x);
+    for (int i = tid; i < sp.pieces; i += 256) M = fmaxf(M, A.part_ml[at + i].x);
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o));
-    const int d = lane * 4;
-    const bool mine = d < A.kv.dim64;
-    v4f acc = v4f{0.f, 0.f, 0.f, 0.f};
-    float L = 0.f;
-    for (int i = wave; i < sp.pieces; i += 4) {
-        const float2 ml = A.part_ml[at + i];
-        if (ml.y == 0.f) continue;   // saw no key
-        const float f = __builtin_amdgcn_exp2f(ml.x - M);
-        L += ml.y * f;
-        if (mine) acc += *(const v4f*)(A.part + (at + i) * A.kv.dim64 + d) * f;
-    }
-    if (mine) *(v4f*)&sums[wave][d] = acc;
-    if (lane == 0) red[wave] = L;
+    if (lane == 0) red[0][wave] = M;
     __syncthreads();
-    if (wave != 0 || !mine) return;
-    L = red[0] + red[1] + red[2] + red[3];
+    M = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+    float L = 0.f;
+    for (int i = tid; i < sp.pieces; i += 256) {
+        const float2 ml = A.part_ml[at + i];
+        const float f = ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - M);   // (a piece without a key for the row)
+        factor[i] = f;
+        L += ml.y * f;
+    }
 #pragma unroll
-    for (int w = 1; w < 4; w++) acc += *(v4f*)&sums[w][d];
+    for (int o = 1; o < 64; o <<= 1) L += __shfl_xor(L, o);
+    if (lane == 0) red[1][wave] = L;
+    __syncthreads();
+    L = red[1][0] + red[1][1] + red[1][2] + red[1][3];
+    const int quads = A.kv.dim64 / 4, groups = 256 / quads, g = tid / quads, d = (tid - g * quads) * 4;   // quads: 16, 32, 48 or 64
+    v4f acc = v4f{0.f, 0.f, 0.f, 0.f};
+    if (g < groups) {
+        const float* from = A.part + at * A.kv.dim64 + d;
+#pragma unroll 4
+        for (int i = g; i < sp.pieces; i += groups) acc += *(const v4f*)(from + (int64_t)i * A.kv.dim64) * factor[i];
+    }
+    sums[tid] = acc;
+    __syncthreads();
+    if (g != 0) return;
+    for (int w = 1; w < groups; w++) acc += sums[w * quads + tid];
     const float inv = L > 0.f ? 1.0f / L : L == L ? 0.f : L;
     RowAt r;
     r.row = row; r.head = head; r.pos = 0; r.live = true;
@@ -632,10 +658,14 @@ int launch_tile(smx_ctx* c, const AttnArgs& A, dim3 grid) {
     hipLaunchKernelGGL((attn_tile_kernel<DC, CT, NT, BF16>), grid, dim3(256), lds, c->stream, A);
     return SMX_OK;
 }
+// Column tiles of a wave: as many as leave two waves a SIMD their registers (queries and sums are 8 CT DC NT and 16 CT DC of 256).
+constexpr int rows_tiles(int dc) { return dc <= 2 ? 2 : 1; }
+constexpr int wave_tiles(int dc) { return dc <= 2 ? 2 : 1; }
 template <int DC>
 int launch_dim(smx_ctx* c, const AttnArgs& A, dim3 grid, bool bf16, int form) {
     if (form == 0) return bf16 ? launch_rows<DC, 1, 1, true>(c, A, grid) : launch_rows<DC, 1, 2, false>(c, A, grid);
-    return bf16 ? launch_tile<DC, 2, 1, true>(c, A, grid) : launch_tile<DC, 2, 2, false>(c, A, grid);
+    if (form == 1) return bf16 ? launch_rows<DC, rows_tiles(DC), 1, true>(c, A, grid) : launch_rows<DC, rows_tiles(DC), 2, false>(c, A, grid);
+    return bf16 ? launch_tile<DC, wave_tiles(DC), 1, true>(c, A, grid) : launch_tile<DC, wave_tiles(DC), 2, false>(c, A, grid);
 }
 
 }  // namespace
@@ -665,19 +695,19 @@ extern "C" int smx_attn_dev(smx_ctx* c, const smx_kv_cache* cache, const smx_kv_
     const size_t per16 = bf16 ? 8 : 4;
     A.vec = cache->head_dim % 16 == 0 && ldq % per16 == 0 && ldo % per16 == 0 && (((uintptr_t)q | (uintptr_t)out) & 15) == 0;
     const size_t tile_rows = batch->max_rows * (size_t)A.group;
-    const int form = tile_rows <= 32 ? 0 : 1;
-    const size_t per_tile = form == 0 ? 16 : 128;
+    const int form = tile_rows <= 16 ? 0 : tile_rows <= 64 ? 1 : 2;
+    const int dc = A.kv.dim64 / 64;
+    const size_t per_tile = form == 0 ? 16 : form == 1 ? 16 * rows_tiles(dc) : 64 * wave_tiles(dc);
     A.row_tiles = (int)((tile_rows + per_tile - 1) / per_tile);
     // tokens in reach of one sequence's rows, and how many workgroups they make without a split
     const size_t reach = window ? std::min<size_t>(A.kv.max_len, window + batch->max_rows + SMX_KV_BLOCK) : (size_t)A.kv.max_len;
     const size_t groups = batch->nseq * cache->kv_heads * (size_t)A.row_tiles;
-    const size_t want = 512;
-    size_t split = groups >= want ? 1 : (want + groups - 1) / groups;
+    const size_t want = 512, least = 128;
+    size_t split = std::min<size_t>(groups >= want ? 1 : (want + groups - 1) / groups, kMaxPieces);
     size_t piece = (std::max<size_t>(reach, 1) + split - 1) / split;
-    piece = std::max<size_t>((piece + 127) & ~size_t(127), 256);
+    piece = std::max<size_t>((piece + 127) & ~size_t(127), least);
     A.piece = (int)std::min<size_t>(piece, size_t(1) << 30);
     A.pieces = (int)std::max<size_t>((reach + piece - 1) / piece, 1);
-    if (A.pieces > 65535 || groups / batch->nseq > INT_MAX) return fail(c, SMX_ERR_LIMIT, "attn_dev: %d pieces of the context", A.pieces);
     if (A.pieces > 1) {
         const size_t n = batch->rows * q_heads * (size_t)A.pieces;
         if ((rc = ensure(c, c->work, n * ((size_t)A.kv.dim64 * 4 + 8))) != SMX_OK) return rc;
@@ -685,7 +715,7 @@ extern "C" int smx_attn_dev(smx_ctx* c, const smx_kv_cache* cache, const smx_kv_
         A.part_ml = (float2*)(A.part + n * A.kv.dim64);
     }
     const dim3 grid((unsigned)(cache->kv_heads * A.row_tiles), (unsigned)A.pieces, (unsigned)batch->nseq);
-    ProfScope ps(c, form == 0 ? "attn_rows" : "attn_tile");
+    ProfScope ps(c, form < 2 ? "attn_rows" : "attn_tile");
     switch (A.kv.dim64 / 64) {
         case 1: rc = launch_dim<1>(c, A, grid, bf16, form); break;
         case 2: rc = launch_dim<2>(c, A, grid, bf16, form); break;
