@@ -310,7 +310,8 @@ int smx_kv_sizes(size_t pages, size_t page_tokens, size_t kv_heads, size_t head_
 int smx_kv_append_dev(smx_ctx* ctx, const smx_kv_cache* cache, const smx_kv_batch* batch, int type, const void* k_dev, size_t ldk,
                       const void* v_dev, size_t ldv, const smx_rope* rope, const void* q_dev, size_t ldq, size_t q_heads,
                       void* q_out_dev, size_t ldqo);
-/* The stored keys and values of the batch's rows as fp32 [rows][kv_heads][head_dim] (either may be NULL). */
+/* The stored keys and values of the batch's rows as fp32 [rows][kv_heads][head_dim] (either may be NULL; rows in front of position
+ * 0 are left as they are). */
 int smx_kv_read_dev(smx_ctx* ctx, const smx_kv_cache* cache, const smx_kv_batch* batch, float* k_dev, float* v_dev);
 /* out = softmax(scale * q K^T) V for each query row and head over the row's own sequence: keys at positions up to the row's own
  * and, with window > 0, only the last `window` of them.  q, out: [rows][q_heads][head_dim] of `type`, ldq, ldo elements from row

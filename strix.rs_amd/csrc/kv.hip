@@ -1,6 +1,7 @@
 // The paged 8-bit key/value cache: a step's keys and values appended with their position rotation, stored values read back.
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include "kv_dev.h"
 
@@ -47,191 +48,346 @@ struct AppendArgs {
     int touched;          // workgroups along x that serve cache blocks; the ones behind them rotate queries
 };
 
-constexpr int kQueryItems = 1024;   // channel pairs per workgroup of the query rotation
+// Channels are worked on W pairs at a time: of 16-byte loads where rows, halves and addresses allow it, else a pair.
+template <bool BF16, bool VEC>
+constexpr int kPairs = VEC ? (BF16 ? 8 : 4) : 1;
+constexpr int kQueryItems = 1024;   // groups of W pairs for each workgroup of the query rotation
 
-// Pair i of a head's dim / 2 channel pairs, rotated: channels *da, *db of the row.  Pairs behind the rotated ones are
-// neighbouring channels that pass through.
-template <bool BF16, bool PAIRS>
-__device__ __forceinline__ float2 rotated_pair(const AppendArgs& A, const void* x, int64_t at, int pos, int i, int* da, int* db) {
+// 2 W channels of a row: a[j], b[j] is pair j of group i (pairs W i ..), rotated.  da, db: channel of a[0], b[0]; the others follow
+// them (PAIRS and channels behind the rotated ones: a[j], b[j] are neighbours, a[j] at da + 2 j).
+template <bool BF16, bool PAIRS, bool VEC>
+struct Group {
+    static constexpr int W = kPairs<BF16, VEC>;
+    float a[W], b[W];
+    int da, db;
+    bool split;   // a and b lie half a rotation apart
+
+    __device__ __forceinline__ void place(int i, int rot) {
+        const int half = rot >> 1;
+        split = !PAIRS && i * W < half;
+        da = split ? i * W : 2 * i * W;
+        db = split ? i * W + half : 2 * i * W + 1;
+    }
+    __device__ __forceinline__ void load(const void* x, int64_t at) {
+        if constexpr (!VEC) {
+            a[0] = load_elem<BF16>(x, at + da);
+            b[0] = load_elem<BF16>(x, at + db);
+        } else {
+            float v[2 * W];
+            const int64_t second = split ? at + db : at + da + W;
+            if constexpr (BF16) {
+                const uint4 p = *(const uint4*)((const uint16_t*)x + at + da), q = *(const uint4*)((const uint16_t*)x + second);
+                const unsigned u[8] = {p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    v[2 * j] = __uint_as_float(u[j] << 16);
+                    v[2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
+                }
+            } else {
+                const float4 p = *(const float4*)((const float*)x + at + da), q = *(const float4*)((const float*)x + second);
+                v[0] = p.x; v[1] = p.y; v[2] = p.z; v[3] = p.w;
+                v[4] = q.x; v[5] = q.y; v[6] = q.z; v[7] = q.w;
+            }
+#pragma unroll
+            for (int j = 0; j < W; j++) {
+                a[j] = split ? v[j] : v[2 * j];
+                b[j] = split ? v[W + j] : v[2 * j + 1];
+            }
+        }
+    }
+    // cs: the position's {cos, sin} of pair 0
+    __device__ __forceinline__ void rotate(const float2* __restrict__ cs, int i, int rot) {
 #pragma clang fp contract(off)
-    const int half = A.rot >> 1;
-    const bool turn = i < half;
-    *da = turn ? (PAIRS ? 2 * i : i) : 2 * i;
-    *db = turn ? (PAIRS ? 2 * i + 1 : i + half) : 2 * i + 1;
-    const float a = load_elem<BF16>(x, at + *da), b = load_elem<BF16>(x, at + *db);
-    if (!turn) return make_float2(a, b);
-    const float2 cs = A.rope[(int64_t)min(pos, A.n_pos - 1) * half + i];
-    return make_float2(a * cs.x - b * cs.y, a * cs.y + b * cs.x);
-}
+        if (i * W >= (rot >> 1)) return;
+        float2 c[W];
+#pragma unroll
+        for (int j = 0; j < W; j++) c[j] = cs[i * W + j];
+#pragma unroll
+        for (int j = 0; j < W; j++) {
+            const float x = a[j], y = b[j];
+            a[j] = x * c[j].x - y * c[j].y;
+            b[j] = x * c[j].y + y * c[j].x;
+        }
+    }
+    // the 2 W channels in memory order: first W at da, the others at second()
+    __device__ __forceinline__ int second() const { return split ? db : da + W; }
+    __device__ __forceinline__ void ordered(float (&v)[2 * W]) const {
+#pragma unroll
+        for (int j = 0; j < W; j++) {
+            if (split) { v[j] = a[j]; v[W + j] = b[j]; }
+            else { v[2 * j] = a[j]; v[2 * j + 1] = b[j]; }
+        }
+    }
+    __device__ __forceinline__ void store(void* y, int64_t at) const {
+        if constexpr (!VEC) {
+            store_elem<BF16>(y, at + da, a[0]);
+            store_elem<BF16>(y, at + db, b[0]);
+        } else {
+            float v[2 * W];
+            ordered(v);
+            if constexpr (BF16) {
+                unsigned u[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) u[j] = f32_to_bf16(v[2 * j]) | (unsigned)f32_to_bf16(v[2 * j + 1]) << 16;
+                *(uint4*)((uint16_t*)y + at + da) = make_uint4(u[0], u[1], u[2], u[3]);
+                *(uint4*)((uint16_t*)y + at + second()) = make_uint4(u[4], u[5], u[6], u[7]);
+            } else {
+                *(float4*)((float*)y + at + da) = make_float4(v[0], v[1], v[2], v[3]);
+                *(float4*)((float*)y + at + second()) = make_float4(v[4], v[5], v[6], v[7]);
+            }
+        }
+    }
+};
 
 // The largest |value| as its bits: NaN and infinity order above every finite value.
 __device__ __forceinline__ unsigned abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
+// Which part of the batch a workgroup serves: block x of those that the sequences' rows lie in, in order.
+struct BlockRows {
+    int s, blk;       // sequence, block
+    int t0, t1;       // the block's tokens that are rows of the batch: [t0, t1), none if t1 <= t0
+    int row;          // row of the block's token 0 (may lie in front of the batch's)
+};
+__device__ __forceinline__ BlockRows block_rows(const KvArgs& a, int x) {
+    BlockRows r;
+    r.s = x;
+    int nth = 0;
+    if (a.row0) {   // a wave looks at 64 sequences at a time
+        const int lane = threadIdx.x & 63;
+        int base = 0, left = x;
+        for (;; base += 64) {
+            if (base >= a.nseq) { r.t0 = r.t1 = 0; r.s = r.blk = r.row = 0; return r; }
+            int n = 0;
+            if (base + lane < a.nseq) {
+                const KvSeq q = kv_seq(a, base + lane);
+                const int first = max(q.len - q.n, 0);
+                n = q.len > first ? (q.len - 1) / SMX_KV_BLOCK - first / SMX_KV_BLOCK + 1 : 0;
+            }
+            int upto = n;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int v = __shfl_up(upto, o);
+                if (lane >= o) upto += v;
+            }
+            const unsigned long long hit = __ballot(upto > left);
+            if (hit) {
+                const int l = __ffsll((long long)hit) - 1;
+                r.s = __builtin_amdgcn_readfirstlane(base + l);
+                nth = __builtin_amdgcn_readfirstlane(left - __shfl(upto - n, l));
+                break;
+            }
+            left -= __shfl(upto, 63);
+        }
+    }
+    const KvSeq q = kv_seq(a, r.s);
+    const int start = q.len - q.n;                 // may be negative: rows in front of position 0 are left out
+    r.blk = max(start, 0) / SMX_KV_BLOCK + nth;
+    r.t0 = max(max(start, 0) - r.blk * SMX_KV_BLOCK, 0);
+    r.t1 = min(q.len - r.blk * SMX_KV_BLOCK, SMX_KV_BLOCK);
+    r.row = q.row + r.blk * SMX_KV_BLOCK - start;
+    return r;
+}
+// Workgroups enough for every block: n rows from the last token of a block on touch (n + 62) / 32.
+int touched_blocks(const smx_kv_batch* b) { return b->row0 ? (int)((b->rows + 62 * b->nseq) / SMX_KV_BLOCK) : (int)b->nseq; }
+
 // Workgroup (x, head, keys | values): x < touched is one block of 32 tokens that the step writes into, the others rotate
-// kQueryItems channel pairs of the queries each (head and z choose among those).
+// kQueryItems groups of channel pairs of the queries each (head and z choose among those).
 //
 // A block is one workgroup's alone, so its scale, the rounding of earlier codes under a scale that grew and the new codes need no
-// atomics: the block's new values go through LDS as fp32, their largest gives the scale, and whole groups of bytes are written
-// (4 tokens of a channel for values, 16 channels of a token for keys).
-template <bool BF16, bool PAIRS>
+// atomics: the block's new values go through LDS as fp32, their largest gives the scale, and the codes leave in the layout's 16-byte
+// units (a token's 16 channels of keys; 8 tokens of 2 channels of values).  In a block that is only partly new, values go by 4 tokens or
+// single bytes, so that nothing is read back unless the scale grew.
+// Bytes bound a prompt chunk (2048 rows of 16 + 16 heads of 256 bf16 channels: 59 MB), the launch a decode step.
+template <bool BF16, bool PAIRS, bool VEC>
 __global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs A) {
 #pragma clang fp contract(off)
-    extern __shared__ float vals[];   // [32][dim + 1]
+    constexpr int W = kPairs<BF16, VEC>;
+    extern __shared__ __align__(16) float vals[];   // [32][pitch]
     __shared__ unsigned red[4];
     const KvArgs& a = A.kv;
-    const int tid = threadIdx.x, half = a.dim >> 1;
+    const int tid = threadIdx.x, groups = a.dim / (2 * W);
+    Group<BF16, PAIRS, VEC> g;
     if ((int)blockIdx.x >= A.touched) {
-        const int64_t items = (int64_t)a.rows * A.q_heads * half;
-        const int64_t group = ((int64_t)(blockIdx.x - A.touched) * gridDim.y + blockIdx.y) * gridDim.z + blockIdx.z;
-        for (int64_t it = group * kQueryItems + tid; it < min((group + 1) * kQueryItems, items); it += 256) {
-            const int64_t rh = it / half;
-            const int row = (int)(rh / A.q_heads), h = (int)(rh - (int64_t)row * A.q_heads), i = (int)(it - rh * half);
-            int s = row;
-            if (a.row0) {   // the last sequence that starts at or before the row
-                int lo = 0, hi = a.nseq - 1;
-                while (lo < hi) {
-                    const int mid = (lo + hi + 1) >> 1;
-                    if (a.row0[mid] <= row) lo = mid; else hi = mid - 1;
+        const int64_t items = (int64_t)a.rows * A.q_heads * groups;
+        const int64_t first = ((((int64_t)blockIdx.x - A.touched) * gridDim.y + blockIdx.y) * gridDim.z + blockIdx.z) * kQueryItems;
+        if (first >= items) return;
+        int row = -1, pos = 0;
+#pragma unroll
+        for (int j = 0; j < kQueryItems / 256; j++) {
+            const int64_t it = first + j * 256 + tid;
+            if (it >= items) return;
+            const unsigned rh = (unsigned)(it / groups);   // rows * q_heads < 2^40: rows are at most 2^24
+            const int i = (int)(it - (int64_t)rh * groups), r = (int)(rh / (unsigned)A.q_heads), h = (int)(rh - (unsigned)r * A.q_heads);
+            if (r != row) {
+                row = r;
+                int s = row;
+                if (a.row0) {   // the last sequence that starts at or before the row
+                    int lo = 0, hi = a.nseq - 1;
+                    while (lo < hi) {
+                        const int mid = (lo + hi + 1) >> 1;
+                        if (a.row0[mid] <= row) lo = mid; else hi = mid - 1;
+                    }
+                    s = lo;
                 }
-                s = lo;
+                const KvSeq q = kv_seq(a, s);
+                pos = max(q.len - q.n + row - q.row, 0);
             }
-            const KvSeq q = kv_seq(a, s);
-            const int pos = max(q.len - q.n + row - q.row, 0);
-            int da, db;
-            const float2 r = rotated_pair<BF16, PAIRS>(A, A.q, (int64_t)row * A.ldq + (int64_t)h * a.dim, pos, i, &da, &db);
-            const int64_t at = (int64_t)row * A.ldqo + (int64_t)h * a.dim;
-            store_elem<BF16>(A.qo, at + da, r.x);
-            store_elem<BF16>(A.qo, at + db, r.y);
+            g.place(i, A.rot);
+            g.load(A.q, (int64_t)row * A.ldq + (int64_t)h * a.dim);
+            if (A.rope) g.rotate(A.rope + (int64_t)min(pos, A.n_pos - 1) * (A.rot >> 1), i, A.rot);
+            g.store(A.qo, (int64_t)row * A.ldqo + (int64_t)h * a.dim);
         }
         return;
     }
-    // which sequence, and which of the blocks that it touches
-    int s = blockIdx.x, nth = 0;
-    if (a.row0) {
-        int left = blockIdx.x;
-        for (s = 0; s < a.nseq; s++) {
-            const KvSeq q = kv_seq(a, s);
-            const int first = max(q.len - q.n, 0);
-            const int blocks = q.len > first ? (q.len - 1) / SMX_KV_BLOCK - first / SMX_KV_BLOCK + 1 : 0;
-            if (left < blocks) break;
-            left -= blocks;
-        }
-        if (s == a.nseq) return;
-        nth = left;
-    }
-    const KvSeq q = kv_seq(a, s);
-    const int start = q.len - q.n;                 // may be negative: rows in front of position 0 are left out
-    const int blk = max(start, 0) / SMX_KV_BLOCK + nth;
-    const int t0 = max(max(start, 0) - blk * SMX_KV_BLOCK, 0), t1 = min(q.len - blk * SMX_KV_BLOCK, SMX_KV_BLOCK);
+    const BlockRows br = block_rows(a, blockIdx.x);
+    const int t0 = br.t0, t1 = br.t1;
     if (t1 <= t0) return;
     const int head = blockIdx.y;
     const bool keys = blockIdx.z == 0;
-    const int64_t bi = kv_block(a, s, head, blk);
-    const int row = q.row + blk * SMX_KV_BLOCK - start;   // of the block's token 0
-    const int pitch = a.dim + 1;
+    const int64_t bi = kv_block(a, br.s, head, br.blk);
+    float* sp = (keys ? a.ks : a.vs) + bi;
+    const float before = t0 > 0 ? *sp : 0.0f;
+    const int pitch = a.dim + 4;
+    const int rot = keys && A.rope ? A.rot : 0;
     unsigned most = 0;
-    const int items = (t1 - t0) * half;
-    for (int it = tid; it < items; it += 256) {
-        const int t = t0 + it / half, i = it % half;
-        float2 r;
-        int da, db;
-        if (keys && A.rope) {
-            r = rotated_pair<BF16, PAIRS>(A, A.k, (int64_t)(row + t) * A.ldk + (int64_t)head * a.dim, blk * SMX_KV_BLOCK + t, i, &da, &db);
+    for (int it = tid; it < (t1 - t0) * groups; it += 256) {
+        const int t = t0 + it / groups, i = it % groups;
+        const int64_t at = (int64_t)(br.row + t) * (keys ? A.ldk : A.ldv) + (int64_t)head * a.dim;
+        g.place(i, rot);
+        g.load(keys ? A.k : A.v, at);
+        if (rot) g.rotate(A.rope + (int64_t)min(br.blk * SMX_KV_BLOCK + t, A.n_pos - 1) * (rot >> 1), i, rot);
+        float v[2 * W];
+        if constexpr (VEC) {
+            g.ordered(v);
+#pragma unroll
+            for (int j = 0; j < 2 * W; j += 4) *(float4*)&vals[t * pitch + (j < W ? g.da + j : g.second() + j - W)] = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
         } else {
-            const int64_t at = (keys ? (int64_t)(row + t) * A.ldk : (int64_t)(row + t) * A.ldv) + (int64_t)head * a.dim;
-            da = 2 * i; db = 2 * i + 1;
-            r = make_float2(load_elem<BF16>(keys ? A.k : A.v, at + da), load_elem<BF16>(keys ? A.k : A.v, at + db));
+            vals[t * pitch + g.da] = g.a[0];
+            vals[t * pitch + g.db] = g.b[0];
         }
-        vals[t * pitch + da] = r.x;
-        vals[t * pitch + db] = r.y;
-        most = max(most, max(abs_bits(r.x), abs_bits(r.y)));
+#pragma unroll
+        for (int j = 0; j < W; j++) most = max(most, max(abs_bits(g.a[j]), abs_bits(g.b[j])));
     }
+#pragma unroll
     for (int o = 1; o < 64; o <<= 1) most = max(most, (unsigned)__shfl_xor((int)most, o));
     if ((tid & 63) == 0) red[tid >> 6] = most;
-    __syncthreads();
+    __syncthreads();   // (every thread has read the old scale, too)
     most = max(max(red[0], red[1]), max(red[2], red[3]));
     const float top = __uint_as_float(most);
     const float fresh = most >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : top >= 0x1p-96f ? top / 127.0f : 0.0f;
-    float* sp = (keys ? a.ks : a.vs) + bi;
     float scale = fresh, ratio = 1.0f;
     bool grown = false;
     if (t0 > 0) {
-        const float before = *sp;
         if (before != before || fresh != fresh) scale = __uint_as_float(0x7fc00000u);
         else if (before < fresh) { ratio = before / fresh; grown = true; }
         else scale = before;
     }
-    __syncthreads();   // every thread has read the old scale
     if (tid == 0) *sp = scale;
     const float inv = scale > 0.0f ? 1.0f / scale : 0.0f;
-    const int w0 = grown ? 0 : t0;   // tokens whose codes change
-    auto code = [&](int t, int d) -> int {
+    // fmin / fmax give the limit for NaN, whose block has inv = 0 and y = NaN throughout: code 0
+    auto code = [&](int t, int d) -> unsigned {
         const float y = rintf(vals[t * pitch + d] * inv);
-        return y == y ? (int)fminf(fmaxf(y, -127.0f), 127.0f) & 255 : 0;
+        return y == y ? (unsigned)(int)fminf(fmaxf(y, -127.0f), 127.0f) & 255u : 0u;
     };
-    auto again = [&](unsigned b) -> int { return (int)rintf((float)(int8_t)b * ratio) & 255; };
+    auto again = [&](unsigned b) -> unsigned { return (unsigned)(int)rintf((float)(int8_t)b * ratio) & 255u; };
+    const int w0 = grown ? 0 : t0;   // tokens whose codes change
     if (keys) {
         int8_t* dst = a.k + bi * (SMX_KV_BLOCK * (int64_t)a.dim64);
-        const int quads = (a.dim + 3) >> 2;
-        for (int it = tid; it < (t1 - w0) * quads; it += 256) {
-            const int t = w0 + it / quads, d = it % quads * 4;
-            unsigned* p = (unsigned*)(dst + kv_k_byte(a.dim64, t, d));
-            unsigned w = 0;
+        // units of 16 channels of a token, in memory order: (token / 16, d / 64, d / 16 % 4, token % 16); all 32 tokens are gone through
+        const int units = 2 * a.dim64;
+        for (int u = tid; u < units; u += 256) {
+            const int c = u >> 6, dc = a.dim64 >> 6, tt = c / dc;
+            const int t = tt * 16 + (u & 15), d0 = (c - tt * dc) * 64 + ((u >> 4) & 3) * 16;
+            if (t < w0 || t >= t1 || d0 >= a.dim) continue;
+            uint4* p = (uint4*)(dst + (int64_t)u * 16);
+            unsigned w[4] = {0, 0, 0, 0};
             if (t < t0) {
-                const unsigned old = *p;
-                for (int j = 0; j < 4; j++) w |= (unsigned)again(old >> (8 * j)) << (8 * j);
+                const uint4 old = *p;
+                const unsigned ow[4] = {old.x, old.y, old.z, old.w};
+#pragma unroll
+                for (int j = 0; j < 16; j++) w[j >> 2] |= again(ow[j >> 2] >> (8 * (j & 3))) << (8 * (j & 3));
             } else {
-                for (int j = 0; j < 4; j++)
-                    if (d + j < a.dim) w |= (unsigned)code(t, d + j) << (8 * j);
+#pragma unroll
+                for (int j = 0; j < 16; j++)
+                    if (VEC || d0 + j < a.dim) w[j >> 2] |= code(t, min(d0 + j, a.dim - 1)) << (8 * (j & 3));
             }
-            *p = w;
+            *p = make_uint4(w[0], w[1], w[2], w[3]);
         }
-    } else {
-        int8_t* dst = a.v + bi * (SMX_KV_BLOCK * (int64_t)a.dim64);
-        const int g0 = w0 >> 2, groups = ((t1 + 3) >> 2) - g0;   // groups of 4 tokens
-        for (int it = tid; it < groups * a.dim; it += 256) {
-            const int t = (g0 + it / a.dim) * 4, d = it % a.dim;
-            unsigned* p = (unsigned*)(dst + kv_v_byte(t, d));
-            unsigned w = 0;
-            const unsigned old = t < t0 ? *p : 0u;
-            for (int j = 0; j < 4; j++) {
-                unsigned b = 0;
-                if (t + j < t0) b = grown ? (unsigned)again(old >> (8 * j)) : (old >> (8 * j)) & 255u;
-                else if (t + j < t1) b = (unsigned)code(t + j, d);
-                w |= b << (8 * j);
+        return;
+    }
+    int8_t* dst = a.v + bi * (SMX_KV_BLOCK * (int64_t)a.dim64);
+    if (t0 == 0 && t1 == SMX_KV_BLOCK) {
+        // units of 8 tokens of channels d and d + 16, in memory order: (d / 32, token / 4 % 4, d % 16)
+        for (int u = tid; u < 2 * a.dim64; u += 256) {
+            const int d = (u >> 6) * 32 + (u & 15), t = ((u >> 4) & 3) * 4;
+            unsigned w[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < 16; j++) {   // (d + 16 of an odd size may be past the head: any code)
+                const int dd = min(d + (j >> 3) * 16, a.dim - 1), tk = t + (j & 3) + ((j >> 2) & 1) * 16;
+                w[j >> 2] |= code(tk, dd) << (8 * (j & 3));
             }
-            *p = w;
+            if (d < a.dim) *(uint4*)(dst + (int64_t)u * 16) = make_uint4(w[0], w[1], w[2], w[3]);
         }
+        return;
+    }
+    const int g0 = w0 >> 2, quads = ((t1 + 3) >> 2) - g0;   // groups of 4 tokens of a channel
+    for (int it = tid; it < quads * a.dim; it += 256) {
+        const int q = it / a.dim, t = (g0 + q) * 4, d = it - q * a.dim;
+        int8_t* p = dst + kv_v_byte(t, d);
+        if (!grown && (t < t0 || t + 4 > t1)) {
+            for (int j = max(t0 - t, 0); j < min(t1 - t, 4); j++) p[j] = (int8_t)code(t + j, d);
+            continue;
+        }
+        unsigned w = 0;
+        const unsigned old = t < t0 ? *(const unsigned*)p : 0u;
+        for (int j = 0; j < 4; j++) {
+            unsigned b = 0;
+            if (t + j < t0) b = again(old >> (8 * j));
+            else if (t + j < t1) b = code(t + j, d);
+            w |= b << (8 * j);
+        }
+        *(unsigned*)p = w;
     }
 }
 
-// Workgroup (row, key/value heads): the stored values of one row.
+// Workgroup (x, head, keys | values): the stored values of one block's rows.  A thread takes 4 tokens of 4 channels, four words of
+// the layout (a token's channels of keys, a channel's tokens of values), so that a wave's stores are whole pieces of rows: the
+// values are four times the bytes of the codes, and 16-byte stores to 64 rows at once took 26 us for 34 MB, these 12.
+template <bool VEC>
 __global__ __launch_bounds__(256) void kv_read_kernel(const KvArgs a, float* __restrict__ k, float* __restrict__ v) {
-    const int row = blockIdx.x;
-    int s = row;
-    if (a.row0) {
-        int lo = 0, hi = a.nseq - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (a.row0[mid] <= row) lo = mid; else hi = mid - 1;
+    const bool keys = blockIdx.z == 0;
+    float* out = keys ? k : v;
+    if (!out) return;
+    const BlockRows br = block_rows(a, blockIdx.x);
+    const int t0 = br.t0, t1 = br.t1, head = blockIdx.y;
+    if (t1 <= t0) return;
+    const int64_t bi = kv_block(a, br.s, head, br.blk);
+    const int8_t* src = (keys ? a.k : a.v) + bi * (SMX_KV_BLOCK * (int64_t)a.dim64);
+    const float scale = (keys ? a.ks : a.vs)[bi];
+    const int64_t ld = (int64_t)a.kv_heads * a.dim;
+    float* base = out + (int64_t)br.row * ld + (int64_t)head * a.dim;   // of the block's token 0
+    const int quads = (a.dim + 3) >> 2;
+    for (int it = threadIdx.x; it < 8 * quads; it += 256) {
+        const int tq = it / quads, t = tq * 4, d = (it - tq * quads) * 4;
+        if (t >= t1 || t + 4 <= t0) continue;
+        unsigned w[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) w[j] = *(const unsigned*)(src + (keys ? kv_k_byte(a.dim64, t + j, d) : kv_v_byte(t, d + j)));
+#pragma unroll
+        for (int j = 0; j < 4; j++) {   // token t + j
+            if (t + j < t0 || t + j >= t1) continue;
+            float f[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) f[i] = (float)(int8_t)(keys ? w[j] >> (8 * i) : w[i] >> (8 * j)) * scale;
+            float* to = base + (t + j) * ld + d;
+            if (VEC) {
+                *(float4*)to = make_float4(f[0], f[1], f[2], f[3]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (d + i < a.dim) to[i] = f[i];
+            }
         }
-        s = lo;
-    }
-    const KvSeq q = kv_seq(a, s);
-    const int pos = q.len - q.n + row - q.row;
-    for (int it = threadIdx.x; it < a.kv_heads * a.dim; it += 256) {
-        const int head = it / a.dim, d = it % a.dim;
-        const int64_t at = (int64_t)row * a.kv_heads * a.dim + it;
-        float kval = 0.f, vval = 0.f;
-        if (pos >= 0 && pos < q.len) {
-            const int64_t bi = kv_block(a, s, head, pos / SMX_KV_BLOCK);
-            const int64_t base = bi * (SMX_KV_BLOCK * (int64_t)a.dim64);
-            const int t = pos % SMX_KV_BLOCK;
-            if (k) kval = (float)a.k[base + kv_k_byte(a.dim64, t, d)] * a.ks[bi];
-            if (v) vval = (float)a.v[base + kv_v_byte(t, d)] * a.vs[bi];
-        }
-        if (k) k[at] = kval;
-        if (v) v[at] = vval;
     }
 }
 
@@ -296,19 +452,28 @@ int smx_kv_append_dev(smx_ctx* c, const smx_kv_cache* cache, const smx_kv_batch*
         A.n_pos = (int)rope->n_pos;
         A.rot = (int)rope->rot_dim;
     }
-    // a sequence of n rows touches at most (n + 61) / 32 blocks
-    A.touched = batch->row0 ? (int)((batch->rows + 61 * batch->nseq) / SMX_KV_BLOCK) : (int)batch->nseq;
+    A.touched = touched_blocks(batch);
+    const bool bf = type == SMX_TYPE_BF16, pairs = rope && rope->interleaved;
+    const size_t W = bf ? 8 : 4, half = rope ? rope->rot_dim / 2 : 0;
+    bool vec = cache->head_dim % (2 * W) == 0 && half % W == 0 && ldk % W == 0 && ldv % W == 0 && (((uintptr_t)k | (uintptr_t)v) & 15) == 0;
+    if (q) vec = vec && ldq % W == 0 && ldqo % W == 0 && (((uintptr_t)q | (uintptr_t)q_out) & 15) == 0;
     size_t extra = 0;
     if (q) {
         A.q = q; A.qo = q_out; A.ldq = (int64_t)ldq; A.ldqo = (int64_t)ldqo; A.q_heads = (int)q_heads;
-        const size_t items = batch->rows * q_heads * (cache->head_dim / 2), per = (size_t)kQueryItems * cache->kv_heads * 2;
+        const size_t items = batch->rows * q_heads * (cache->head_dim / (vec ? 2 * W : 2)), per = (size_t)kQueryItems * cache->kv_heads * 2;
         extra = (items + per - 1) / per;
     }
+    if (batch->rows * q_heads >= (size_t(1) << 31) || A.touched + extra > INT_MAX)
+        return fail(c, SMX_ERR_LIMIT, "kv_append_dev: %zu rows of %zu query heads", batch->rows, q_heads);
     const dim3 grid((unsigned)(A.touched + extra), (unsigned)cache->kv_heads, 2);
-    const size_t lds = SMX_KV_BLOCK * (cache->head_dim + 1) * 4;
+    const size_t lds = SMX_KV_BLOCK * (cache->head_dim + 4) * 4;
     ProfScope ps(c, "kv_append");
-    const bool bf = type == SMX_TYPE_BF16, pairs = rope && rope->interleaved;
-    auto kern = bf ? (pairs ? kv_append_kernel<true, true> : kv_append_kernel<true, false>) : (pairs ? kv_append_kernel<false, true> : kv_append_kernel<false, false>);
+    auto pick = [&](auto bf16, auto two) {
+        return vec ? kv_append_kernel<decltype(bf16)::value, decltype(two)::value, true> : kv_append_kernel<decltype(bf16)::value, decltype(two)::value, false>;
+    };
+    std::true_type yes;
+    std::false_type no;
+    auto kern = bf ? (pairs ? pick(yes, yes) : pick(yes, no)) : (pairs ? pick(no, yes) : pick(no, no));
     hipLaunchKernelGGL(kern, grid, dim3(256), lds, c->stream, A);
     SMX_HIP(c, hipGetLastError());
     return SMX_OK;
@@ -322,7 +487,9 @@ int smx_kv_read_dev(smx_ctx* c, const smx_kv_cache* cache, const smx_kv_batch* b
     if (batch->nseq == 0 || batch->rows == 0) return SMX_OK;
     if (!k && !v) return fail(c, SMX_ERR_ARG, "kv_read_dev: nothing to read into");
     ProfScope ps(c, "kv_read");
-    hipLaunchKernelGGL(kv_read_kernel, dim3((unsigned)batch->rows), dim3(256), 0, c->stream, a, k, v);
+    const bool vec = cache->head_dim % 4 == 0 && (((uintptr_t)k | (uintptr_t)v) & 15) == 0;
+    hipLaunchKernelGGL(vec ? kv_read_kernel<true> : kv_read_kernel<false>, dim3((unsigned)touched_blocks(batch), (unsigned)cache->kv_heads, 2), dim3(256), 0,
+                       c->stream, a, k, v);
     SMX_HIP(c, hipGetLastError());
     return SMX_OK;
 }

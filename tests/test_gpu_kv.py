@@ -108,6 +108,30 @@ def test_append_equals_its_definition(accel, pkg, ty, dim, rot, pairs, page, kv,
             r += n
 
 
+@pytest.mark.parametrize("off", [0, 1, 30, 31])
+@pytest.mark.parametrize("n", [1, 2, 3, 31, 32, 33, 34, 35, 65, 66])
+def test_every_block_that_rows_touch(accel, pkg, off, n):
+    """One sequence whose rows begin and end at every kind of place in a block."""
+    rng = np.random.default_rng(off * 100 + n)
+    kv, dim, page = 1, 64, 32
+    cache = R.Cache(6, page, kv, dim)
+    table = R.tables(rng, 6, page, [off + n])
+    R.append(cache, table, [0], [off], *(rng.standard_normal((off, kv, dim)).astype(np.float32) for _ in range(2)))
+    k, kr, _ = _rows(rng, "f32", n, kv, dim)
+    v, vr, _ = _rows(rng, "f32", n, kv, dim)
+    with R.Dev(accel) as dev:
+        d = R.OnDevice(pkg, dev, cache)
+        batch = d.batch(table, [off + n], [n], always_row0=True)
+        accel.kv_append_dev(d.handle, batch, dev.put(kr), dev.put(vr))
+        R.append(cache, table, [off], [n], k, v)
+        ko, vo = dev.room(kr.nbytes), dev.room(vr.nbytes)
+        accel.kv_read_dev(d.handle, batch, ko, vo)
+        got = d.planes()
+        assert _same(got[2], cache.ks) and _same(got[3], cache.vs)
+        assert np.array_equal(dev.get(ko, k.shape)[:, 0], cache.tokens("k", table[0], 0, off + n)[off:])
+        assert np.array_equal(dev.get(vo, v.shape)[:, 0], cache.tokens("v", table[0], 0, off + n)[off:])
+
+
 def test_append_without_rotation_or_queries_in_place_queries(accel, pkg):
     rng = np.random.default_rng(5)
     kv, dim, rows = 2, 64, 3
