@@ -45,6 +45,7 @@ struct AttnArgs {
     int piece;          // tokens per piece (a multiple of 32)
     int pieces;         // of the longest sequence
     int row_tiles;
+    int paired;         // (see attn_tile_kernel)
     float scale;        // times log2(e)
     int vec;            // rows may be read and written 16 bytes (bf16: 8) at a time
 };
@@ -85,14 +86,25 @@ __device__ __forceinline__ int64_t uniform(int64_t v) {
     return (int64_t)((uint64_t)hi << 32 | lo);
 }
 
-// Largest of the four lanes that share a row (lane, lane ^ 16, lane ^ 32, lane ^ 48), and their sum.
+// The two values whose larger (sum) a step of a reduction over the four lanes of a row (lane, ^ 16, ^ 32, ^ 48) takes: rows of 16 lanes, or
+// halves, swapped between two copies.
+__device__ __forceinline__ float2 swap32(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return make_float2(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float2 swap16(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return make_float2(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
 __device__ __forceinline__ float row_max(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16));
-    return fmaxf(v, __shfl_xor(v, 32));
+    float2 s = swap32(v);
+    s = swap16(fmaxf(s.x, s.y));
+    return fmaxf(s.x, s.y);
 }
 __device__ __forceinline__ float row_sum(float v) {
-    v += __shfl_xor(v, 16);
-    return v + __shfl_xor(v, 32);
+    float2 s = swap32(v);
+    s = swap16(s.x + s.y);
+    return s.x + s.y;
 }
 
 // The query rows of one column tile as the B operand of S^T = K Q^T: lane (row lane % 16, g) holds channels 64 c + 16 g + 0..15 of
@@ -203,10 +215,15 @@ __device__ __forceinline__ void rescale(const float (&mx)[CT], float (&m)[CT], f
 template <int NT>
 __device__ __forceinline__ void split_prob(const float (&p)[8], v8h (&pf)[NT]) {
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        const _Float16 hi = (_Float16)p[j];
-        pf[0][j] = hi;
-        if (NT == 2) pf[NT - 1][j] = (_Float16)(p[j] - (float)hi);
+    for (int j = 0; j < 8; j += 2) {
+        const v2h hi = {(_Float16)p[j], (_Float16)p[j + 1]};   // one packed conversion
+        pf[0][j] = hi[0];
+        pf[0][j + 1] = hi[1];
+        if (NT == 2) {   // p - hi is exact; an FMA takes the f16 operand as it is
+            const v2h lo = {(_Float16)fmaf((float)hi[0], -1.0f, p[j]), (_Float16)fmaf((float)hi[1], -1.0f, p[j + 1])};
+            pf[NT - 1][j] = lo[0];
+            pf[NT - 1][j + 1] = lo[1];
+        }
     }
 }
 
@@ -426,18 +443,24 @@ __global__ __launch_bounds__(256, CT == 2 ? 2 : DC <= 1 ? 4 : DC == 2 ? 3 : 2) v
 }
 
 // ---- many rows: a prompt chunk.  Workgroup (head and tile of 64 CT rows, piece, sequence); a wave holds 16 CT rows, and the four
-// share tiles of 64 tokens that are widened to f16 on their way into LDS (each byte once per workgroup).  The next tile's bytes are
-// in flight while one is computed.
+// share tiles of TB blocks that are widened to f16 on their way into LDS (each byte once per workgroup), two of them in turn; the tile
+// behind the next one is in flight in registers.
+// A block's scores are formed one step ahead: the matrix unit works on the next block's while the vector unit turns this block's into
+// probabilities (exp, two f16 terms: about ten instructions a score, as long as the matrix instructions of the score take).
 template <int DC, int CT, int NT, bool BF16>
 __global__ __launch_bounds__(256, 2) void attn_tile_kernel(const AttnArgs A) {
-    constexpr int D64 = DC * 64, NO = DC * 4, KF = DC * 2;
+    constexpr int D64 = DC * 64, NO = DC * 4, KF = DC * 2, TB = DC <= 2 ? 2 : 1;
+    constexpr int UNITS = TB * 2 * DC, PER = (UNITS + 3) / 4;      // 1 KB units of a tile's keys (and values); of them a wave's
+    constexpr int KEYS = TB * 2 * KF * 64, TILE = KEYS + TB * NO * 64;   // 16-byte words: keys [block][token / 16][KF][lane], values [block][NO][lane]
     __shared__ Segment seg;
-    extern __shared__ uint4 stage[];   // keys [4 token tiles][KF][64 lanes], values [2 blocks][NO][64 lanes], 8 f16 each
-    uint4* kt = stage;
-    uint4* vt = stage + 4 * KF * 64;
+    extern __shared__ uint4 stage[];   // [2][TILE]
     const int s = blockIdx.z, piece = blockIdx.y;
     const int kvh = blockIdx.x % A.kv.kv_heads;
-    const int tile = A.row_tiles - 1 - blockIdx.x / A.kv.kv_heads;   // the longest rows first
+    // The longest rows first.  Where every workgroup has a place at once (two on a CU), the second half goes the other way round, so that
+    // each CU has a long and a short one.
+    int tile = blockIdx.x / A.kv.kv_heads;
+    if (!A.paired || tile < (A.row_tiles + 1) / 2) tile = A.row_tiles - 1 - tile;
+    else tile -= (A.row_tiles + 1) / 2;
     const Span sp = seq_span(A, s);
     const int rows = sp.q.n * A.group, row0 = tile * 64 * CT;
     if (row0 >= rows) return;
@@ -464,14 +487,13 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(const AttnArgs A) {
         for (int i = 0; i < NO; i++) o[ct][i] = v4f{0.f, 0.f, 0.f, 0.f};
     }
     // this wave's rows: every one sees [all_lo, all_hi]; none sees a token outside [any_lo, any_hi]
-    const bool wlive = wrow0 < rows;
     const int wfirst = pos0 + wrow0 / A.group, wlast = pos0 + min(wrow0 + 16 * CT - 1, rows - 1) / A.group;
     const int all_hi = wfirst, all_lo = A.window > 0 ? wlast - A.window + 1 : 0;
-    const int any_hi = wlast, any_lo = A.window > 0 ? wfirst - A.window + 1 : 0;
+    const int any_hi = wrow0 < rows ? wlast : -1, any_lo = A.window > 0 ? wfirst - A.window + 1 : 0;
     int vexp = 0;
     const int b0 = tok0 / SMX_KV_BLOCK, b1 = tok1 > tok0 ? (tok1 + SMX_KV_BLOCK - 1) / SMX_KV_BLOCK : b0;
     for (int c0 = b0; c0 < b1; c0 += kSegBlocks) {
-        const int n = min(kSegBlocks, b1 - c0);
+        const int n = min(kSegBlocks, b1 - c0), tiles = (n + TB - 1) / TB;
         __syncthreads();
         load_segment<256>(A, seg, s, kvh, c0, n);
         __syncthreads();
@@ -484,46 +506,45 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(const AttnArgs A) {
             vexp = e;
         }
         const float vup = pow2(vexp);
-        // thread's share of a tile: 16-byte units u = tid + 256 j of the 2 blocks' 4 DC units of keys and of values each
-        uint4 kb[DC], vb[DC];
-        auto fetch = [&](int i) {
+        uint4 kb[PER], vb[PER];
+        // this wave's units of a tile: u = wave + 4 j (a last tile's missing block is its first again, and masked)
+        auto fetch = [&](int t) {
 #pragma unroll
-            for (int j = 0; j < DC; j++) {
-                const int u = wave + 4 * j;                 // 1 KB unit of the tile: block u / (2 DC)
-                const int64_t base = seg.place[min(i + u / (2 * DC), n - 1)] * (SMX_KV_BLOCK * D64) + (u % (2 * DC)) * 1024 + lane * 16;
-                kb[j] = *(const uint4*)(A.kv.k + base);
-                vb[j] = *(const uint4*)(A.kv.v + base);
+            for (int j = 0; j < PER; j++) {
+                const int u = wave + 4 * j;
+                if (UNITS % 4 && u >= UNITS) break;
+                const int64_t base = uniform(seg.place[min(t * TB + u / (2 * DC), n - 1)]) * (SMX_KV_BLOCK * D64) + (u % (2 * DC)) * 1024;
+                kb[j] = *(const uint4*)(A.kv.k + base + (unsigned)lane * 16);
+                vb[j] = *(const uint4*)(A.kv.v + base + (unsigned)lane * 16);
             }
         };
-        fetch(0);
-        for (int i = 0; i < n; i += 2) {
-            if (i) __syncthreads();   // the tile in front has been used
+        auto put = [&](int t) {
+            uint4* to = stage + (t & 1) * TILE + lane;
 #pragma unroll
-            for (int j = 0; j < DC; j++) {
+            for (int j = 0; j < PER; j++) {
                 const int u = wave + 4 * j;
-                // keys: unit (block, token tile, c) -> token tile 2 block + tt, chunks 2 c and 2 c + 1
-                uint4* kd = kt + ((u / DC) * KF + (u % DC) * 2) * 64 + lane;
+                if (UNITS % 4 && u >= UNITS) break;
+                uint4* kd = to + ((u / DC) * KF + (u % DC) * 2) * 64;     // (block, token / 16), chunk d / 64 -> fragments 2 c, 2 c + 1
                 kd[0] = __builtin_bit_cast(uint4, widen8(kb[j].x, kb[j].y));
                 kd[64] = __builtin_bit_cast(uint4, widen8(kb[j].z, kb[j].w));
-                uint4* vd = vt + (2 * u) * 64 + lane;       // values: unit (block, d / 32) -> channel tiles 2 (d / 32), + 1
+                uint4* vd = to + KEYS + (2 * u) * 64;                     // (block, d / 32) -> channel tiles 2 (d / 32), + 1
                 vd[0] = __builtin_bit_cast(uint4, widen8(vb[j].x, vb[j].y));
                 vd[64] = __builtin_bit_cast(uint4, widen8(vb[j].z, vb[j].w));
             }
-            __syncthreads();
-            if (i + 2 < n) fetch(i + 2);
+        };
+        auto needed = [&](int i) {
             const int tok = (c0 + i) * SMX_KV_BLOCK;
-            if (!wlive || tok > any_hi || tok + 2 * SMX_KV_BLOCK <= any_lo) continue;
-            const bool edge = tok + 2 * SMX_KV_BLOCK - 1 > all_hi || tok < all_lo || tok + 2 * SMX_KV_BLOCK > tok1;   // (an odd last block stands in the tile twice)
-            const float ks[2] = {seg.ks[i], seg.ks[min(i + 1, n - 1)]};
-            const float vs[2] = {seg.vs[i] * vup, seg.vs[min(i + 1, n - 1)] * vup};
-            v4f sc[CT][4];
+            return i < n && tok <= any_hi && tok + SMX_KV_BLOCK > any_lo;
+        };
+        auto scores = [&](v4f (&sc)[CT][2], int i) {
+            const uint4* kt = stage + ((i / TB) & 1) * TILE + (i % TB) * 2 * KF * 64 + lane;
 #pragma unroll
-            for (int tt = 0; tt < 4; tt++) {
-#pragma unroll
-                for (int ct = 0; ct < CT; ct++) sc[ct][tt] = v4f{0.f, 0.f, 0.f, 0.f};
+            for (int tt = 0; tt < 2; tt++) {
                 v8h kf[KF];
 #pragma unroll
-                for (int k = 0; k < KF; k++) kf[k] = __builtin_bit_cast(v8h, kt[(tt * KF + k) * 64 + lane]);
+                for (int k = 0; k < KF; k++) kf[k] = __builtin_bit_cast(v8h, kt[(tt * KF + k) * 64]);
+#pragma unroll
+                for (int ct = 0; ct < CT; ct++) sc[ct][tt] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int nt = NT - 1; nt >= 0; nt--)   // the small terms first: fewer roundings of large sums
 #pragma unroll
@@ -531,51 +552,138 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(const AttnArgs A) {
 #pragma unroll
                         for (int ct = 0; ct < CT; ct++) sc[ct][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[k], qf[ct][nt][k], sc[ct][tt], 0, 0, 0);
             }
-            float mx[CT];
+        };
+        // probabilities times value scale of block i, 2^(scores * f + base), and their product with its values; the sums of
+        // probabilities take the scale out again (per_vs)
+        auto weigh = [&](const v4f (&sc)[CT][2], const float (&f)[CT], const float (&base)[CT], float per_vs, float poison, int i) {
+            v8h pf[CT][NT];
 #pragma unroll
             for (int ct = 0; ct < CT; ct++) {
+                float p[8], sum = 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    p[j] = __builtin_amdgcn_exp2f(fmaf(sc[ct][j >> 2][j & 3], f[ct], base[ct]));
+                    sum += p[j];
+                }
+                l[ct] = fmaf(sum, per_vs, l[ct]) + (sum > 0.f ? poison : 0.f);
+                split_prob<NT>(p, pf[ct]);
+            }
+            const uint4* vt = stage + ((i / TB) & 1) * TILE + KEYS + (i % TB) * NO * 64 + lane;
+#pragma unroll
+            for (int k = 0; k < NO; k++) {
+                const v8h vf = __builtin_bit_cast(v8h, vt[k * 64]);
+#pragma unroll
+                for (int nt = NT - 1; nt >= 0; nt--)
+#pragma unroll
+                    for (int ct = 0; ct < CT; ct++) o[ct][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[ct][nt], o[ct][k], 0, 0, 0);
+            }
+        };
+        // scores(nxt, i + 1) and weigh(cur, i) in one, in the order the instructions are to leave: a pair of probabilities between every
+        // MS matrix instructions of the next block's scores, then the product with the values.  The operands pass through a ring of KF
+        // registers' worth of LDS reads, each asked for when the one in its place has been used last.
+        auto both = [&](const v4f (&cur)[CT][2], v4f (&nxt)[CT][2], const float (&f)[CT], const float (&base)[CT], float per_vs, float poison, int i) {
+            constexpr int TT = KF * NT * CT, MS = 2 * TT / (4 * CT);   // matrix instructions of 16 tokens; between two pairs
+            const uint4* kt = stage + (((i + 1) / TB) & 1) * TILE + ((i + 1) % TB) * 2 * KF * 64 + lane;
+            const uint4* vt = stage + ((i / TB) & 1) * TILE + KEYS + (i % TB) * NO * 64 + lane;
+            v8h ring[KF], pf[CT][NT];
+            float sum[CT];
+#pragma unroll
+            for (int k = 0; k < KF; k++) ring[k] = __builtin_bit_cast(v8h, kt[k * 64]);
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++) {
+                sum[ct] = 0.f;
+                nxt[ct][0] = nxt[ct][1] = v4f{0.f, 0.f, 0.f, 0.f};
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int pair = 0; pair < 4 * CT; pair++) {
+                const int pc = pair % CT, j = pair / CT * 2;
+                float p[2];
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    p[h] = __builtin_amdgcn_exp2f(fmaf(cur[pc][(j + h) >> 2][(j + h) & 3], f[pc], base[pc]));
+                    sum[pc] += p[h];
+                }
+                const v2h hi = {(_Float16)p[0], (_Float16)p[1]};
+                pf[pc][0][j] = hi[0];
+                pf[pc][0][j + 1] = hi[1];
+                if (NT == 2) {
+                    const v2h lo = {(_Float16)fmaf((float)hi[0], -1.0f, p[0]), (_Float16)fmaf((float)hi[1], -1.0f, p[1])};
+                    pf[pc][NT - 1][j] = lo[0];
+                    pf[pc][NT - 1][j + 1] = lo[1];
+                }
+#pragma unroll
+                for (int q = pair * MS; q < pair * MS + MS; q++) {
+                    const int tt = q / TT, r = q % TT, nt = NT - 1 - r / (KF * CT), k = r / CT % KF, ct = r % CT;
+                    nxt[ct][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ring[k], qf[ct][nt][k], nxt[ct][tt], 0, 0, 0);
+                    if (nt == 0 && ct == CT - 1) ring[k] = __builtin_bit_cast(v8h, tt == 0 ? kt[(KF + k) * 64] : vt[k * 64]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++) l[ct] = fmaf(sum[ct], per_vs, l[ct]) + (sum[ct] > 0.f ? poison : 0.f);
+#pragma unroll
+            for (int k = 0; k < NO; k++) {
+#pragma unroll
+                for (int nt = NT - 1; nt >= 0; nt--)
+#pragma unroll
+                    for (int ct = 0; ct < CT; ct++) o[ct][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ring[k % KF], pf[ct][nt], o[ct][k], 0, 0, 0);
+                if (k + KF < NO) ring[k % KF] = __builtin_bit_cast(v8h, vt[(k + KF) * 64]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        // block i, whose scores are in `cur`; the next block's go to `nxt`
+        auto step = [&](v4f (&cur)[CT][2], v4f (&nxt)[CT][2], int i) {
+            if (i % TB == TB - 1 && i / TB + 1 < tiles) {
+                __syncthreads();   // everyone is done with the tile in front of this one
+                put(i / TB + 1);
+                if (i / TB + 2 < tiles) fetch(i / TB + 2);
+                __syncthreads();
+            }
+            const bool now = needed(i), then = needed(i + 1);
+            if (!now) {
+                if (then) scores(nxt, i + 1);
+                return;
+            }
+            const int tok = (c0 + i) * SMX_KV_BLOCK;
+            const bool edge = tok + SMX_KV_BLOCK - 1 > all_hi || tok < all_lo;
+            const float ks = seg.ks[i];
+            // a value scale of 0 stands for codes of 0; a NaN one is for the rows that see a token of the block
+            const float scale = seg.vs[i] * vup, vs = fmaxf(scale, 0x1p-60f), poison = scale == scale ? 0.f : scale;
+            const float log_vs = __builtin_amdgcn_logf(vs), per_vs = __builtin_amdgcn_rcpf(vs);
+            float f[CT], base[CT], mx[CT];
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++) {
+                f[ct] = unit[ct] * ks;
+                if (edge) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const int key = tok + 16 * (j >> 2) + 4 * g + (j & 3);
+                        const bool out = key > at[ct].pos || (A.window > 0 && key <= at[ct].pos - A.window);
+                        cur[ct][j >> 2][j & 3] = out ? -INFINITY : cur[ct][j >> 2][j & 3] * f[ct];
+                    }
+                    f[ct] = 1.0f;
+                }
                 mx[ct] = kNoMax;
 #pragma unroll
-                for (int tt = 0; tt < 4; tt++) {
-                    const float f = unit[ct] * ks[tt >> 1];
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        sc[ct][tt][j] *= f;
-                        if (edge) {
-                            const int key = tok + 16 * tt + 4 * g + j;
-                            if (key > at[ct].pos || key >= tok1 || (A.window > 0 && key <= at[ct].pos - A.window)) sc[ct][tt][j] = -INFINITY;
-                        }
-                        mx[ct] = fmaxf(mx[ct], sc[ct][tt][j]);
-                    }
-                }
-                mx[ct] = row_max(mx[ct]);
+                for (int j = 0; j < 8; j++) mx[ct] = fmaxf(mx[ct], cur[ct][j >> 2][j & 3]);
+                mx[ct] = row_max(mx[ct]) * f[ct];
             }
             rescale<CT, NO>(mx, m, l, o);
 #pragma unroll
-            for (int b = 0; b < 2; b++) {
-                v8h pf[CT][NT];
-#pragma unroll
-                for (int ct = 0; ct < CT; ct++) {
-                    float p[8], sum = 0.f;
-#pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        const float t = sc[ct][2 * b + (j >> 2)][j & 3];
-                        const float e2 = __builtin_amdgcn_exp2f(t - m[ct]);
-                        sum += e2;
-                        p[j] = edge && t == -INFINITY ? 0.f : e2 * vs[b];
-                    }
-                    l[ct] += sum;
-                    split_prob<NT>(p, pf[ct]);
-                }
-#pragma unroll
-                for (int k = 0; k < NO; k++) {
-                    const v8h vf = __builtin_bit_cast(v8h, vt[(b * NO + k) * 64 + lane]);
-#pragma unroll
-                    for (int ct = 0; ct < CT; ct++)
-#pragma unroll
-                        for (int nt = NT - 1; nt >= 0; nt--) o[ct][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[ct][nt], o[ct][k], 0, 0, 0);
-                }
-            }
+            for (int ct = 0; ct < CT; ct++) base[ct] = log_vs - m[ct];
+            if (then) both(cur, nxt, f, base, per_vs, poison, i);
+            else weigh(cur, f, base, per_vs, poison, i);
+        };
+        fetch(0);
+        put(0);
+        if (tiles > 1) fetch(1);
+        __syncthreads();
+        v4f s0[CT][2], s1[CT][2];
+        if (needed(0)) scores(s0, 0);
+        for (int i = 0; i < n; i += 2) {
+            step(s0, s1, i);
+            if (i + 1 < n) step(s1, s0, i + 1);
         }
     }
     const float down = pow2(-vexp);
@@ -652,7 +760,7 @@ int launch_rows(smx_ctx* c, const AttnArgs& A, dim3 grid) {
 }
 template <int DC, int CT, int NT, bool BF16>
 int launch_tile(smx_ctx* c, const AttnArgs& A, dim3 grid) {
-    const size_t lds = (4 * DC * 2 + 2 * DC * 4) * 1024;
+    const size_t lds = 2 * (DC <= 2 ? 2 : 1) * (2 * DC * 2 + DC * 4) * 1024;
     int rc;
     if ((rc = set_dyn_lds(c, attn_tile_kernel<DC, CT, NT, BF16>, lds)) != SMX_OK) return rc;
     hipLaunchKernelGGL((attn_tile_kernel<DC, CT, NT, BF16>), grid, dim3(256), lds, c->stream, A);
@@ -714,6 +822,7 @@ extern "C" int smx_attn_dev(smx_ctx* c, const smx_kv_cache* cache, const smx_kv_
         A.part = (float*)c->work.p;
         A.part_ml = (float2*)(A.part + n * A.kv.dim64);
     }
+    A.paired = groups * (size_t)A.pieces <= 2 * (size_t)c->num_cu && A.pieces == 1;
     const dim3 grid((unsigned)(cache->kv_heads * A.row_tiles), (unsigned)A.pieces, (unsigned)batch->nseq);
     ProfScope ps(c, form < 2 ? "attn_rows" : "attn_tile");
     switch (A.kv.dim64 / 64) {
