@@ -376,7 +376,7 @@ void smx_destroy(smx_ctx* c) {
         free_weight(kv.second.up);
         free_weight(kv.second.down);
     }
-    for (DevBuf* b : {&c->xf32, &c->xq, &c->xd, &c->xs, &c->yf32, &c->work, &c->work2, &c->tab, &c->raw})
+    for (DevBuf* b : {&c->xf32, &c->xq, &c->xd, &c->xs, &c->yf32, &c->work, &c->work2, &c->counts, &c->tab, &c->raw})
         if (b->p) (void)hipFree(b->p);
     for (char* p : c->retired) (void)hipFree(p);
     for (DevBuf* b : {&c->hx, &c->hy, &c->htab})

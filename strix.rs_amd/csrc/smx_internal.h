@@ -74,6 +74,7 @@ struct smx_ctx {
     smx::DevBuf yf32;   // staged outputs
     smx::DevBuf work;   // split-K partials, MoE intermediates, dumps
     smx::DevBuf work2;
+    smx::DevBuf counts; // counters of the few-row attention, 0 between its launches
     smx::DevBuf tab;    // small tables (ids, weights, tile tables)
     smx::DevBuf raw;    // upload staging: the raw GGUF blocks of the tensor being repacked (kept up to kRawKeepBytes between uploads)
     smx::DevBuf hx, hy; // pinned HOST staging of the host-pointer calls' activations and results
