@@ -12,8 +12,9 @@
 //   4  one workgroup for each row sorts the list (up to kList tokens), which places the cut at one token, finds the chunk that
 //      the pick falls into from the totals and the pick in the chunk
 // A row is read three times (without top_k and top_p: twice), every other launch from its end, where the one in front has left
-// the caches.  A list that does not fit (thousands of equal logits at the cut, or a cut more than kReach below the largest logit) is
-// found by bisection over the logits instead.
+// the caches.  256 rows of 262144 (268 MB) with top_p: 52 + 66 + 63 + 11 us; one row with top_k and top_p:
+// 4 + 8 + 4 + 4.  A list that does not fit (thousands of equal logits at the cut, or a cut more than kReach below the largest logit)
+// is found by bisection over the logits instead.
 #include <algorithm>
 #include <climits>
 #include <cmath>
@@ -66,33 +67,29 @@ __device__ __forceinline__ unsigned key_of(float x) {
 }
 __device__ __forceinline__ float of_key(unsigned k) { return k == 0 ? -INFINITY : __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
-// Division of distances by a row's temperature, correctly rounded, in three operations where the general one takes eleven: with
+// (x - max) / T, correctly rounded, in five operations where the general division alone takes eleven: with a = x - max,
 // r = RN(1 / T), q = RN(a r) is within one unit of a / T, the remainder a - q T is exact in an FMA, and RN(q + remainder r) is the
-// correctly rounded quotient (Markstein's theorem, for divisors whose mantissa is not all ones).  Quotients below -200 keep q (their
-// exponential is 0); remainders lose bits to underflow only where |a / T| < 2^-40 (exponential 1).
+// correctly rounded quotient (Markstein's theorem, for divisors whose mantissa is not all ones).  Distances of more than 200 T count
+// as 200 T (exp(-200) is 0 in fp32, and so are the exponentials of all beyond); remainders lose bits to underflow only where
+// |a / T| < 2^-40 (exponential 1).  A largest logit of +inf has distance 0 from itself and so a share.
 struct Temp {
-    float T, r;
+    float mx, T, r, far;
     bool quick;
 };
-__device__ __forceinline__ Temp temp_of(float T) {
+__device__ __forceinline__ Temp temp_of(float T, float mx) {
     const unsigned b = __float_as_uint(T);
-    return Temp{T, 1.0f / T, T > 0x1p-60f && T < 0x1p60f && (b & 0x7fffffu) != 0x7fffffu};
+    return Temp{mx, T, 1.0f / T, -200.0f * T, T > 0x1p-60f && T < 0x1p60f && (b & 0x7fffffu) != 0x7fffffu && mx < INFINITY};
 }
-__device__ __forceinline__ float over_T(float a, const Temp& t) {
+__device__ __forceinline__ float depth(float x, const Temp& t) {
 #pragma clang fp contract(off)
-    if (!t.quick) return a / t.T;   // (the same for the whole row)
-    const float q = a * t.r;
-    return q > -200.0f ? fmaf(fmaf(-q, t.T, a), t.r, q) : q;
+    if (!t.quick) return x == t.mx ? 0.0f : (x - t.mx) / t.T;   // (the same for the whole row)
+    const float a = __builtin_amdgcn_fmed3f(x - t.mx, t.far, 0.0f), q = a * t.r;
+    return fmaf(fmaf(-q, t.T, a), t.r, q);
 }
-// (x - max) / T of a candidate (x > -inf), 0 for the largest (so that a +inf maximum has a share)
-__device__ __forceinline__ float depth(float x, float mx, const Temp& t) {
-#pragma clang fp contract(off)
-    return x == mx ? 0.0f : over_T(x - mx, t);
-}
-// floor(e * 2^40) of an e in [0, 1], from its bits
+// floor(e * 2^40) of an e in [0, 1]: below 2^52, so the low bits of the double 2^52 + it are the number (shifts of 64 bits by e's
+// exponent instead: launch 2 with 256 rows of 262144 71 us, with this 65)
 __device__ __forceinline__ unsigned long long weight(float e) {
-    const unsigned b = __float_as_uint(e);
-    return ((unsigned long long)((b & 0x7fffffu) | 0x800000u) << 17) >> min(127u - (b >> 23), 63u);
+    return __builtin_bit_cast(unsigned long long, (double)truncf(e * 0x1p40f) + 0x1p52) & 0xfffffffffffffull;
 }
 // Bin of a depth: steps of distance below the largest logit.  Every rounding is monotone in x, so a smaller bin means a larger logit.
 __device__ __forceinline__ int bin_of(float z) {
@@ -146,8 +143,8 @@ struct Ask {
     float mx, top_p, min_p;
     Temp T, bin_T;    // bin_T divides distances for bin_of: T, or 1 where tokens are counted
     int top_k;
-    __device__ float share(float x) const { return expf(depth(x, mx, T)); }
-    __device__ int bin(float x) const { return bin_of(depth(x, mx, bin_T)); }
+    __device__ float share(float x) const { return expf(depth(x, T)); }
+    __device__ int bin(float x) const { return bin_of(depth(x, bin_T)); }
 };
 __device__ __forceinline__ Ask ask_of(const SampleArgs& A, int row) {
     // every wave reads the parts' candidates for itself: no barrier
@@ -159,13 +156,13 @@ __device__ __forceinline__ Ask ask_of(const SampleArgs& A, int row) {
     q.best_at = ~(unsigned)b;
     q.mx = of_key(top);
     const float T = A.temperature ? A.temperature[row] : 1.0f;
-    q.T = temp_of(T);
+    q.T = temp_of(T, q.mx);
     q.top_k = A.top_k ? A.top_k[row] : 0;
     q.top_p = A.top_p ? A.top_p[row] : 1.0f;
     q.min_p = A.min_p ? fminf(A.min_p[row], 1.0f) : 0.0f;
     const bool k = q.top_k > 0 && q.top_k < A.vocab;
     q.mode = top == 0 ? kNone : !(T > 0.0f) || q.top_k == 1 || q.top_p <= 0.0f ? kGreedy : k ? kTopK : q.top_p < 1.0f ? kTopP : kFree;
-    q.bin_T = q.mode == kTopK ? Temp{1.0f, 1.0f, true} : q.T;
+    q.bin_T = q.mode == kTopK ? temp_of(1.0f, q.mx) : q.T;
     return q;
 }
 
@@ -243,7 +240,8 @@ __device__ __forceinline__ float floor_of_bin(const Ask& q, int bin) {
 }
 
 // Launch 2.  Workgroup (part, row), from the last to the first.  The last one of a row to finish reads the whole histogram: the
-// cut's bin is the first whose running total reaches top_k tokens, or floor(top_p * all weight).
+// cut's bin is the first whose running total reaches top_k tokens, or floor(top_p * all weight).  256 rows of 262144: 66 us, 50 of
+// them the reading, 10 the LDS atomics.
 __global__ __launch_bounds__(1024) void sample_hist_kernel(const SampleArgs A) {
     __shared__ unsigned long long hist[kBins], red[16];
     __shared__ unsigned done;
@@ -259,10 +257,9 @@ __global__ __launch_bounds__(1024) void sample_hist_kernel(const SampleArgs A) {
         load_chunk(x, c, v);
 #pragma unroll
         for (int n = 0; n < 16; n++) {
-            if (!(v[n] > -INFINITY)) continue;
-            const float z = depth(v[n], q.mx, q.bin_T);
+            const float z = depth(v[n], q.bin_T);
             const unsigned long long w = q.mode == kTopK ? 1ull : weight(expf(z));
-            if (w) atomicAdd(&hist[bin_of(z)], w);
+            if (w && v[n] > -INFINITY) atomicAdd(&hist[bin_of(z)], w);
         }
     }
     __syncthreads();
@@ -274,7 +271,7 @@ __global__ __launch_bounds__(1024) void sample_hist_kernel(const SampleArgs A) {
     }
     // What passes between workgroups is atomic at device scope, performed where all XCDs see it: this thread's additions are
     // waited for, then the workgroup counts itself; the reads below are atomic too.  (A fence by each wave would write its XCD's L2
-    // back: 256 rows of 262144 329 us instead of 75.)
+    // back: 256 rows of 262144 329 us instead of 66.)
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (threadIdx.x == 0) done = atomicAdd(&cut->done, 1u);
@@ -319,8 +316,10 @@ __global__ __launch_bounds__(1024) void sample_hist_kernel(const SampleArgs A) {
     if (threadIdx.x == 0) { cut->above = above; cut->limit = limit; }
 }
 
-// Launch 3.  Workgroup (part, row).
-__global__ __launch_bounds__(1024) void sample_gather_kernel(const SampleArgs A) {
+// Launch 3.  Workgroup (part, row).  Tokens below the cut's bin take one comparison, the ones above it an exponential, the bin's own
+// (few) an LDS atomic.  256 rows of 262144 with top_p: 63 us, of which 45 are the reading; with the scalar registers for one
+// workgroup a CU (no second bound) 83.
+__global__ __launch_bounds__(1024, 8) void sample_gather_kernel(const SampleArgs A) {
     __shared__ unsigned long long list[kList];
     __shared__ unsigned found, start;
     const int row = blockIdx.y, part = blockIdx.x, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, lane = threadIdx.x & 63;
@@ -330,42 +329,27 @@ __global__ __launch_bounds__(1024) void sample_gather_kernel(const SampleArgs A)
     __syncthreads();
     // (NaN: none; top_k rows list everything that they keep)
     const float total_from = q.mode == kFree ? -3.402823466e38f : A.cuts[row].total_from;
-    const float list_from = q.mode == kFree ? __uint_as_float(0x7fc00000u) : A.cuts[row].list_from;
+    const float list_from = q.mode == kFree ? total_from : A.cuts[row].list_from;
     const Row x = row_of(A, row);
     const int c1 = min((part + 1) * A.part_chunks, A.chunks);
     for (int c = part * A.part_chunks + wave; c < c1; c += waves) {
         float v[16];
         load_chunk(x, c, v);
         const int first = first_of(x, c);
-        unsigned put = 0;
+        double sum = 0;   // of 16 whole numbers up to 2^40: exact
 #pragma unroll
-        for (int n = 0; n < 16; n++) put |= (v[n] >= list_from && !(v[n] >= total_from) ? 1u : 0u) << n;
-        if (__ballot(put != 0)) {   // the wave's share of the workgroup's list: one LDS atomic for a chunk
-            const int mine = __popc(put);
-            int upto = mine;
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const int r = __shfl_up(upto, o);
-                if (lane >= o) upto += r;
-            }
-            int at = 0;
-            if (lane == 63) at = (int)atomicAdd(&found, (unsigned)upto);
-            at = __shfl(at, 63) + upto - mine;
-            for (unsigned left = put; left; left &= left - 1, at++) {
-                if (at >= kList) break;
-                const int i = token_of(first, __ffs(left) - 1);
-                list[at] = (unsigned long long)~key_of(x.x[i]) << 32 | (unsigned)i;
-            }
-        }
-        if (q.mode != kTopK) {
-            double sum = 0;   // of 16 whole numbers up to 2^40: exact
-#pragma unroll
-            for (int n = 0; n < 16; n++) {
+        for (int n = 0; n < 16; n++) {
+            if (v[n] >= list_from) {
                 if (v[n] >= total_from) {
                     const float e = q.share(v[n]);
                     if (e >= q.min_p) sum += (double)truncf(e * 0x1p40f);
+                } else {
+                    const unsigned at = atomicAdd(&found, 1u);
+                    if (at < (unsigned)kList) list[at] = (unsigned long long)~key_of(v[n]) << 32 | (unsigned)token_of(first, n);
                 }
             }
+        }
+        if (q.mode != kTopK) {
             const unsigned long long total = wave_sum((unsigned long long)sum);
             if (lane == 0) A.totals[(int64_t)row * A.chunks + c] = total;
         }
