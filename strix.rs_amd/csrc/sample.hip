@@ -277,13 +277,13 @@ __global__ __launch_bounds__(1024) void sample_hist_kernel(const SampleArgs A) {
     if (threadIdx.x == 0) done = atomicAdd(&cut->done, 1u);
     __syncthreads();
     if (done != (unsigned)A.parts - 1) return;
-    const int per = kBins / blockDim.x;   // neighbouring bins for each thread: 2..8
-    unsigned long long bins[8], sum = 0;
+    const int per = kBins / blockDim.x;   // neighbouring bins for each thread: 2 or 4
+    unsigned long long bins[4], sum = 0;
 #pragma unroll
-    for (int j = 0; j < 8; j++)   // (all in flight at once)
+    for (int j = 0; j < 4; j++)   // (all in flight at once)
         bins[j] = j < per ? __hip_atomic_load(&all[threadIdx.x * per + j], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
+    for (int j = 0; j < 4; j++) {
         if (j < per) hist[threadIdx.x * per + j] = bins[j];
         sum += bins[j];
     }
@@ -801,13 +801,14 @@ int launch_sample(smx_ctx* c, const float* logits, size_t rows, size_t vocab, si
     A.chunks = (int)((vocab + skew + kChunk - 1) / kChunk);
     if (p) { A.temperature = p->temperature; A.top_k = p->top_k; A.top_p = p->top_p; A.min_p = p->min_p; }
     A.u = u; A.ids = ids; A.prob = prob;
-    // Parts of a row: 512 workgroups in all (two a CU), of at least one chunk a wave.  Few rows take workgroups of 4 waves, so that
-    // a single row spreads over as many CUs as it has chunks for.
-    const bool few = rows * (size_t)A.chunks < 512 * 16;
-    const int threads = few ? 256 : 1024;
-    const size_t want = 512, most = ((size_t)A.chunks + threads / 64 - 1) / (threads / 64);
+    // Parts of a row: 512 workgroups in all (two a CU), of at least one chunk a wave.  Workgroups of 8 waves where a call is small: more
+    // of them for a row, though each adds a histogram to the row's; of 16 where there is work for all of them anyhow.  4 / 8 / 16 waves,
+    // us of the four launches with top_p: 1 x 131072 26.4 / 26.0 / 28.3, 16 x 131072 34.0 / 30.7 / 33.4, 32 x 131072
+    // 42.8 / 37.9 / 38.3, 64 x 131072 55.6 / 48.2 / 46.6, 64 x 32000 31.7 / 29.2 / 31.7.
+    const int threads = rows * (size_t)A.chunks < 4096 ? 512 : 1024;
+    const size_t waves = threads / 64, want = 512, most = ((size_t)A.chunks + waves - 1) / waves;
     size_t parts = std::max<size_t>(1, std::min(most, (want + rows - 1) / rows));
-    const size_t waves = threads / 64;   // whole rounds of the waves
+    // whole rounds of the waves
     A.part_chunks = (int)std::max<size_t>(waves, ((A.chunks + parts - 1) / parts + waves / 2) / waves * waves);
     A.parts = (A.chunks + A.part_chunks - 1) / A.part_chunks;
     // workspace of up to kRowsAtOnce rows (the launches of a larger call follow one another)
