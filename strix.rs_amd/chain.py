@@ -10,8 +10,10 @@ Per layer, four calls / five launches:
                                launch                                                     d, logits -> y[hidden] (+ ids[k], w[k])
 (route="call": the router as smx_moe_router_dev, route="launches": as smx_gemv_dev + smx_moe_route_dev, each followed by
 smx_moe_ffn_routed_dev: six launches, same bits.)
-Attention, RoPE and the KV cache are outside this path.  The benchmark (bench.py) and the parity test
-(tests/test_gpu_chain.py) both run this class, so what is measured is what is checked.
+The benchmark (bench.py) and the parity test (tests/test_gpu_chain.py) both run this class, so what is measured is what is checked.
+
+AttentionChain is the other half, for a batch of sequences: projections, the paged cache and the attention over it, and the sampled
+token at the end (the reference's rope, append and sdpa of decode.rs:1136-1180, 5326-5368).  tests/test_gpu_attention_chain.py runs it.
 """
 
 
@@ -76,6 +78,86 @@ class FfnMoeChain:
         return self.layers * (5 if self.route == "in_launch" else 6)
 
     def close(self):
+        for p in self._bufs:
+            self.acc.dev_free(p)
+        self._bufs = []
+
+
+class AttentionChain:
+    """The attention half of a decoder stack and the sampled end of a step, for a batch of sequences over paged 8-bit caches.
+
+    Per layer:
+        1. rmsnorm + quantiser + q, k and v projections  x -> q, k, v   (one row: one launch; more: a launch and a GEMM each)
+        2. smx_kv_append_dev   q and k rotated, k and v into the layer's cache
+        3. smx_attn_dev        q over the cache -> o
+        4. smx_gemv_dev        quantiser + output projection            o -> y[hidden]
+    and behind the last layer rmsnorm + lm_head and smx_sample_dev on the rows that the caller names.
+
+    Each call's rows, lengths and page table are a KvBatch of the caller's, whose device arrays the kernels read when they run: a
+    captured decode step (one row for each sequence) serves every later one, with new lengths and pages written in front of it.
+
+    pkg: the package module (its KvCache, KvBatch and Rope); keys(l) -> (q, k, v, o) weight keys of layer l; rows: the most that one
+    call brings.  keep_stages: every layer gets buffers of its own, so that a test can read each stage back."""
+
+    def __init__(self, pkg, acc, layers, hidden, q_heads, kv_heads, head_dim, keys, lm_head, vocab, norm_w_dev, rows, pages, page_tokens, max_pos,
+                 rope_base=1e4, window=0, eps=1e-6, keep_stages=False):
+        self.pkg, self.acc, self.layers, self.hidden, self.keys = pkg, acc, layers, hidden, keys
+        self.q_heads, self.kv_heads, self.head_dim = q_heads, kv_heads, head_dim
+        self.lm_head, self.vocab, self.norm_w_dev, self.rows, self.window, self.eps = lm_head, vocab, norm_w_dev, rows, window, eps
+        self._bufs = []
+        code_bytes, scales = pkg.kv_sizes(pages, page_tokens, kv_heads, head_dim)
+        self.cache = [pkg.KvCache(pages, page_tokens, kv_heads, head_dim, self._alloc(code_bytes), self._alloc(code_bytes), self._alloc(scales * 4),
+                                  self._alloc(scales * 4)) for _ in range(layers)]
+        table = self._alloc(max_pos * head_dim * 4)
+        acc.rope_table_dev(rope_base, head_dim, max_pos, table)
+        self.rope = pkg.Rope(table, max_pos, head_dim)
+        qw, kw = rows * q_heads * head_dim * 4, rows * kv_heads * head_dim * 4
+        self.stage = [{"q": self._alloc(qw), "k": self._alloc(kw), "v": self._alloc(kw), "o": self._alloc(qw)} for _ in range(layers if keep_stages else 1)]
+        self.y = [self._alloc(rows * hidden * 4) for _ in range(layers if keep_stages else 2)]
+        self.logits = self._alloc(rows * vocab * 4)
+
+    def _alloc(self, nbytes):
+        p = self.acc.dev_alloc(nbytes)
+        self._bufs.append(p)
+        return p
+
+    def buffers(self, l):
+        """(stage buffers, output buffer) of layer l."""
+        return self.stage[l % len(self.stage)], self.y[l % len(self.y)]
+
+    def _project(self, keys, x_dev, rows, outs):
+        """rmsnorm of rows of x_dev through the projections `keys`."""
+        if rows == 1:
+            return self.acc.gemv_fused_dev(list(keys), self.pkg.ACT_RMSNORM, x_dev, self.norm_w_dev, list(outs), self.eps)
+        return all([self.acc.gemm_fused_dev(k, self.pkg.ACT_RMSNORM, x_dev, self.norm_w_dev, rows, y, self.eps) for k, y in zip(keys, outs)])
+
+    def enqueue(self, x_dev, batch):
+        """Enqueue all layers for the rows of `batch` on the context's stream (capturable once a call of the same sizes has run); returns the
+        device buffer holding the last layer's output."""
+        acc, cur = self.acc, x_dev
+        if batch.rows > self.rows:
+            raise ValueError(f"{batch.rows} rows, buffers for {self.rows}")
+        for l in range(self.layers):
+            b, y = self.buffers(l)
+            q, k, v, o = self.keys(l)
+            ok = self._project((q, k, v), cur, batch.rows, (b["q"], b["k"], b["v"]))
+            if ok:
+                acc.kv_append_dev(self.cache[l], batch, b["k"], b["v"], rope=self.rope, q=b["q"], q_heads=self.q_heads, q_out=b["q"])
+                acc.attn_dev(self.cache[l], batch, b["q"], self.q_heads, self.head_dim ** -0.5, b["o"], window=self.window)
+                ok = (acc.gemv_dev if batch.rows <= 32 else acc.gemm_dev)(o, b["o"], batch.rows, y)
+            if not ok:
+                raise RuntimeError(f"layer {l}: a weight of the chain is not resident")
+            cur = y
+        return cur
+
+    def sample(self, y_dev, rows, u_dev, ids_dev, temperature=None, top_k=None, top_p=None, min_p=None, prob=None):
+        """Enqueue rmsnorm, the lm_head and the pick of one token for each of `rows` rows of hidden states (device arrays throughout)."""
+        if not self._project((self.lm_head,), y_dev, rows, (self.logits,)):
+            raise RuntimeError("the lm_head is not resident")
+        self.acc.sample_dev(self.logits, rows, self.vocab, u_dev, ids_dev, temperature, top_k, top_p, min_p, prob)
+
+    def close(self):
+        self.acc.sync()
         for p in self._bufs:
             self.acc.dev_free(p)
         self._bufs = []
