@@ -338,6 +338,13 @@ int launch_dim(smx_ctx* c, const AttnArgs& A, dim3 grid, bool bf16) {
 
 using namespace smx;
 
+// Tokens that are worth a second workgroup on a CU (a workgroup's start and its share of the join cost as much as some 200).  us at one
+// workgroup a CU / two, with the pieces' tokens.  Few rows (24 of 80 channels, 4 key/value heads): 1 sequence of 16000 tokens
+// 18.2 / 20.5 (256 / 128), 5 of 4000 18.9 / 20.3 (384 / 256), 20 of 4000 31.1 / 31.0 (1408 / 768), 5 of 16000 29.7 / 29.2
+// (1408 / 640); 72 rows, 20 of 16000 174 / 120.  Many rows (40 tokens of 32 heads of 128 channels, 8 key/value heads): 1 of 4000
+// 27.8 / 31.0 (256 / 128), 1 of 16000 47 / 40 (1024 / 512), 4 of 4000 52 / 45 (1024 / 512).
+constexpr size_t kWorthFew = 512, kWorthMany = 256;
+
 extern "C" int smx_attn_dev(smx_ctx* c, const smx_kv_cache* cache, const smx_kv_batch* batch, int type, const void* q, size_t ldq, size_t q_heads,
                             float scale, size_t window, void* out, size_t ldo) {
     if (!c) return SMX_ERR_ARG;
@@ -368,10 +375,12 @@ extern "C" int smx_attn_dev(smx_ctx* c, const smx_kv_cache* cache, const smx_kv_
     A.row_tiles = (int)((tile_rows + A.tile_rows - 1) / A.tile_rows);
     // how many workgroups the sequences make without a split
     const size_t groups = batch->nseq * cache->kv_heads * (size_t)A.row_tiles;
-    const size_t want = 512, least = 128;
-    size_t split = std::min<size_t>(groups >= want ? 1 : (want + groups - 1) / groups, kMaxPieces);
-    size_t piece = (std::max<size_t>(reach, 1) + split - 1) / split;
-    piece = std::max<size_t>((piece + 127) & ~size_t(127), least);
+    // one to a CU, or two where that leaves each enough tokens; never a few more than that, which would wait for a round of their own
+    const size_t cus = c->num_cu, span = std::max<size_t>(reach, 1);
+    size_t split = std::max<size_t>(1, cus / groups);
+    if (2 * cus / groups > split && span / (2 * cus / groups) >= (few ? kWorthFew : kWorthMany)) split = 2 * cus / groups;
+    split = std::min<size_t>(split, kMaxPieces);
+    const size_t piece = std::max<size_t>(((span + split - 1) / split + 127) & ~size_t(127), 128);
     A.piece = (int)std::min<size_t>(piece, size_t(1) << 30);
     A.pieces = (int)std::max<size_t>((reach + piece - 1) / piece, 1);
     if (A.pieces > 1) {
