@@ -51,7 +51,7 @@ struct AppendArgs {
 // Channels are worked on W pairs at a time: of 16-byte loads where rows, halves and addresses allow it, else a pair.
 template <bool BF16, bool VEC>
 constexpr int kPairs = VEC ? (BF16 ? 8 : 4) : 1;
-constexpr int kQueryItems = 1024;   // groups of W pairs for each workgroup of the query rotation
+constexpr int kQueryItems = 512;   // groups of W pairs for each workgroup of the query rotation
 
 // 2 W channels of a row: a[j], b[j] is pair j of group i (pairs W i ..), rotated.  da, db: channel of a[0], b[0]; the others follow
 // them (PAIRS and channels behind the rotated ones: a[j], b[j] are neighbours, a[j] at da + 2 j).
@@ -59,6 +59,8 @@ template <bool BF16, bool PAIRS, bool VEC>
 struct Group {
     static constexpr int W = kPairs<BF16, VEC>;
     float a[W], b[W];
+    float2 c[W];
+    uint4 p, q;
     int da, db;
     bool split;   // a and b lie half a rotation apart
 
@@ -68,25 +70,37 @@ struct Group {
         da = split ? i * W : 2 * i * W;
         db = split ? i * W + half : 2 * i * W + 1;
     }
-    __device__ __forceinline__ void load(const void* x, int64_t at) {
+    // asked for: the channels' bytes, and the position's {cos, sin} of the group's pairs (cs: of pair 0; group i is one of the rotated)
+    __device__ __forceinline__ void fetch(const void* x, int64_t at) {
+        const int64_t second = VEC && !split ? at + da + W : at + db;
+        if constexpr (VEC) {
+            p = BF16 ? *(const uint4*)((const uint16_t*)x + at + da) : *(const uint4*)((const float*)x + at + da);
+            q = BF16 ? *(const uint4*)((const uint16_t*)x + second) : *(const uint4*)((const float*)x + second);
+        } else {
+            p.x = BF16 ? ((const uint16_t*)x)[at + da] : ((const unsigned*)x)[at + da];
+            q.x = BF16 ? ((const uint16_t*)x)[second] : ((const unsigned*)x)[second];
+        }
+    }
+    __device__ __forceinline__ void fetch_turn(const float2* __restrict__ cs, int i) {
+#pragma unroll
+        for (int j = 0; j < W; j++) c[j] = cs[i * W + j];
+    }
+    // what has been asked for, as numbers
+    __device__ __forceinline__ void open() {
         if constexpr (!VEC) {
-            a[0] = load_elem<BF16>(x, at + da);
-            b[0] = load_elem<BF16>(x, at + db);
+            a[0] = __uint_as_float(BF16 ? p.x << 16 : p.x);
+            b[0] = __uint_as_float(BF16 ? q.x << 16 : q.x);
         } else {
             float v[2 * W];
-            const int64_t second = split ? at + db : at + da + W;
-            if constexpr (BF16) {
-                const uint4 p = *(const uint4*)((const uint16_t*)x + at + da), q = *(const uint4*)((const uint16_t*)x + second);
-                const unsigned u[8] = {p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
+            const unsigned u[8] = {p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
+            for (int j = 0; j < 8; j++) {
+                if constexpr (BF16) {
                     v[2 * j] = __uint_as_float(u[j] << 16);
                     v[2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
+                } else {
+                    v[j] = __uint_as_float(u[j]);
                 }
-            } else {
-                const float4 p = *(const float4*)((const float*)x + at + da), q = *(const float4*)((const float*)x + second);
-                v[0] = p.x; v[1] = p.y; v[2] = p.z; v[3] = p.w;
-                v[4] = q.x; v[5] = q.y; v[6] = q.z; v[7] = q.w;
             }
 #pragma unroll
             for (int j = 0; j < W; j++) {
@@ -95,13 +109,8 @@ struct Group {
             }
         }
     }
-    // cs: the position's {cos, sin} of pair 0
-    __device__ __forceinline__ void rotate(const float2* __restrict__ cs, int i, int rot) {
+    __device__ __forceinline__ void turn() {
 #pragma clang fp contract(off)
-        if (i * W >= (rot >> 1)) return;
-        float2 c[W];
-#pragma unroll
-        for (int j = 0; j < W; j++) c[j] = cs[i * W + j];
 #pragma unroll
         for (int j = 0; j < W; j++) {
             const float x = a[j], y = b[j];
@@ -194,48 +203,61 @@ int touched_blocks(const smx_kv_batch* b) { return b->row0 ? (int)((b->rows + 62
 // kQueryItems groups of channel pairs of the queries each (head and z choose among those).
 //
 // A block is one workgroup's alone, so its scale, the rounding of earlier codes under a scale that grew and the new codes need no
-// atomics: the block's new values go through LDS as fp32, their largest gives the scale, and the codes leave in the layout's 16-byte
-// units (a token's 16 channels of keys; 8 tokens of 2 channels of values).  In a block that is only partly new, values go by 4 tokens or
-// single bytes, so that nothing is read back unless the scale grew.
-// Bytes bound a prompt chunk (2048 rows of 16 + 16 heads of 256 bf16 channels: 59 MB), the launch a decode step.
+// atomics: the block's new values stay in registers, their largest gives the scale, and the codes go through LDS (in the layout's
+// order) to leave in its 16-byte units (a token's 16 channels of keys; 8 tokens of 2 channels of values).  In a block that is only
+// partly new, values go by 4 tokens or single bytes, so that nothing is read back unless the scale grew.
+// Bytes bound a prompt chunk (2048 rows of 16 + 16 heads of 256 bf16 channels, 59 MB: 17 us, 20 with the new values in LDS as fp32 and
+// loads asked for one group at a time), the launch and a chain of three loads (the step's arrays, its rows, the page) a decode step
+// (64 rows of 32 + 16 heads of 128: 5.8 us): what does not depend on another load is asked for in front of it.
 template <bool BF16, bool PAIRS, bool VEC>
 __global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs A) {
 #pragma clang fp contract(off)
-    constexpr int W = kPairs<BF16, VEC>;
-    extern __shared__ __align__(16) float vals[];   // [32][pitch]
+    constexpr int W = kPairs<BF16, VEC>, ROUNDS = SMX_KV_BLOCK * SMX_KV_MAX_HEAD_DIM / (2 * W * 256), TURNS = kQueryItems / 256;
+    extern __shared__ __align__(16) int8_t image[];   // [SMX_KV_BLOCK * dim64]: the block's new codes
     __shared__ unsigned red[4];
     const KvArgs& a = A.kv;
     const int tid = threadIdx.x, groups = a.dim / (2 * W);
-    Group<BF16, PAIRS, VEC> g;
     if ((int)blockIdx.x >= A.touched) {
         const int64_t items = (int64_t)a.rows * A.q_heads * groups;
         const int64_t first = ((((int64_t)blockIdx.x - A.touched) * gridDim.y + blockIdx.y) * gridDim.z + blockIdx.z) * kQueryItems;
         if (first >= items) return;
-        int row = -1, pos = 0;
+        // (one division of 64 bits for the workgroup, the threads' own are of 32)
+        const unsigned per_row = (unsigned)A.q_heads * (unsigned)groups;   // < 2^23
+        const int r0 = (int)(first / per_row);
+        const unsigned i0 = (unsigned)(first - (int64_t)r0 * per_row), left = (unsigned)min(items - first, (int64_t)kQueryItems);
+        Group<BF16, PAIRS, VEC> g[TURNS];
+        int row[TURNS], head[TURNS], nth[TURNS];
 #pragma unroll
-        for (int j = 0; j < kQueryItems / 256; j++) {
-            const int64_t it = first + j * 256 + tid;
-            if (it >= items) return;
-            const unsigned rh = (unsigned)(it / groups);   // rows * q_heads < 2^40: rows are at most 2^24
-            const int i = (int)(it - (int64_t)rh * groups), r = (int)(rh / (unsigned)A.q_heads), h = (int)(rh - (unsigned)r * A.q_heads);
-            if (r != row) {
-                row = r;
-                int s = row;
+        for (int j = 0; j < TURNS; j++) {   // (a thread without an item takes the last one and stores nothing)
+            const unsigned it = i0 + min(j * 256u + tid, left - 1), over = it / per_row, in = it - over * per_row;
+            row[j] = r0 + (int)over;
+            head[j] = (int)(in / (unsigned)groups);
+            nth[j] = (int)in - head[j] * groups;
+            g[j].place(nth[j], A.rot);
+            g[j].fetch(A.q, (int64_t)row[j] * A.ldq + (int64_t)head[j] * a.dim);
+        }
+        if (A.rope) {
+#pragma unroll
+            for (int j = 0; j < TURNS; j++) {
+                int s = row[j];
                 if (a.row0) {   // the last sequence that starts at or before the row
                     int lo = 0, hi = a.nseq - 1;
                     while (lo < hi) {
                         const int mid = (lo + hi + 1) >> 1;
-                        if (a.row0[mid] <= row) lo = mid; else hi = mid - 1;
+                        if (a.row0[mid] <= row[j]) lo = mid; else hi = mid - 1;
                     }
                     s = lo;
                 }
                 const KvSeq q = kv_seq(a, s);
-                pos = max(q.len - q.n + row - q.row, 0);
+                const int pos = max(q.len - q.n + row[j] - q.row, 0);
+                if (nth[j] * W < A.rot >> 1) g[j].fetch_turn(A.rope + (int64_t)min(pos, A.n_pos - 1) * (A.rot >> 1), nth[j]);
             }
-            g.place(i, A.rot);
-            g.load(A.q, (int64_t)row * A.ldq + (int64_t)h * a.dim);
-            if (A.rope) g.rotate(A.rope + (int64_t)min(pos, A.n_pos - 1) * (A.rot >> 1), i, A.rot);
-            g.store(A.qo, (int64_t)row * A.ldqo + (int64_t)h * a.dim);
+        }
+#pragma unroll
+        for (int j = 0; j < TURNS; j++) {
+            g[j].open();
+            if (A.rope && nth[j] * W < A.rot >> 1) g[j].turn();
+            if (j * 256u + tid < left) g[j].store(A.qo, (int64_t)row[j] * A.ldqo + (int64_t)head[j] * a.dim);
         }
         return;
     }
@@ -244,29 +266,31 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs A) {
     if (t1 <= t0) return;
     const int head = blockIdx.y;
     const bool keys = blockIdx.z == 0;
+    const int rot = keys && A.rope ? A.rot : 0, n = (t1 - t0) * groups;
+    Group<BF16, PAIRS, VEC> g[ROUNDS];
+    int tok[ROUNDS], nth[ROUNDS];
+#pragma unroll
+    for (int j = 0; j < ROUNDS; j++) {   // (a thread without an item takes the last one again)
+        if (j * 256 >= n) continue;
+        const int it = min(j * 256 + tid, n - 1);
+        tok[j] = t0 + it / groups;
+        nth[j] = it - (tok[j] - t0) * groups;
+        g[j].place(nth[j], rot);
+        g[j].fetch(keys ? A.k : A.v, (int64_t)(br.row + tok[j]) * (keys ? A.ldk : A.ldv) + (int64_t)head * a.dim);
+        if (nth[j] * W < rot >> 1) g[j].fetch_turn(A.rope + (int64_t)min(br.blk * SMX_KV_BLOCK + tok[j], A.n_pos - 1) * (rot >> 1), nth[j]);
+    }
     const int64_t bi = kv_block(a, br.s, head, br.blk);
     float* sp = (keys ? a.ks : a.vs) + bi;
     const float before = t0 > 0 ? *sp : 0.0f;
-    const int pitch = a.dim + 4;
-    const int rot = keys && A.rope ? A.rot : 0;
+    for (int u = tid; u < 2 * a.dim64; u += 256) ((uint4*)image)[u] = make_uint4(0, 0, 0, 0);
     unsigned most = 0;
-    for (int it = tid; it < (t1 - t0) * groups; it += 256) {
-        const int t = t0 + it / groups, i = it % groups;
-        const int64_t at = (int64_t)(br.row + t) * (keys ? A.ldk : A.ldv) + (int64_t)head * a.dim;
-        g.place(i, rot);
-        g.load(keys ? A.k : A.v, at);
-        if (rot) g.rotate(A.rope + (int64_t)min(br.blk * SMX_KV_BLOCK + t, A.n_pos - 1) * (rot >> 1), i, rot);
-        float v[2 * W];
-        if constexpr (VEC) {
-            g.ordered(v);
 #pragma unroll
-            for (int j = 0; j < 2 * W; j += 4) *(float4*)&vals[t * pitch + (j < W ? g.da + j : g.second() + j - W)] = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-        } else {
-            vals[t * pitch + g.da] = g.a[0];
-            vals[t * pitch + g.db] = g.b[0];
-        }
+    for (int j = 0; j < ROUNDS; j++) {
+        if (j * 256 >= n) continue;
+        g[j].open();
+        if (nth[j] * W < rot >> 1) g[j].turn();
 #pragma unroll
-        for (int j = 0; j < W; j++) most = max(most, max(abs_bits(g.a[j]), abs_bits(g.b[j])));
+        for (int w = 0; w < W; w++) most = max(most, max(abs_bits(g[j].a[w]), abs_bits(g[j].b[w])));
     }
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) most = max(most, (unsigned)__shfl_xor((int)most, o));
@@ -284,11 +308,36 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs A) {
     }
     if (tid == 0) *sp = scale;
     const float inv = scale > 0.0f ? 1.0f / scale : 0.0f;
-    // fmin / fmax give the limit for NaN, whose block has inv = 0 and y = NaN throughout: code 0
-    auto code = [&](int t, int d) -> unsigned {
-        const float y = rintf(vals[t * pitch + d] * inv);
-        return y == y ? (unsigned)(int)fminf(fmaxf(y, -127.0f), 127.0f) & 255u : 0u;
-    };
+    // round-half-even(v * inv) within +-127 as the low byte of 1.5 * 2^23 + it (a block without inv has codes of 0: the image as it is; one
+    // with it holds finite values only)
+    auto code = [&](float v) -> unsigned { return __float_as_uint(__builtin_amdgcn_fmed3f(v * inv, -127.0f, 127.0f) + 12582912.0f); };
+#pragma unroll
+    for (int j = 0; j < ROUNDS; j++) {
+        if (j * 256 >= n || inv == 0.0f) continue;
+        const int t = tok[j];
+        float v[2 * W];
+        g[j].ordered(v);
+#pragma unroll
+        for (int h = 0; h < 2; h++) {   // W channels in memory order from d on (VEC: of one 16)
+            const int d = h == 0 ? g[j].da : VEC ? g[j].second() : g[j].db;
+            unsigned b[W];
+#pragma unroll
+            for (int w = 0; w < W; w++) b[w] = code(v[h * W + w]);
+            if (!keys) {
+                int8_t* to = &image[kv_v_byte(t, d)];   // (of one 16: 16 bytes from channel to channel)
+#pragma unroll
+                for (int w = 0; w < W; w++) to[w * 16] = (int8_t)b[w];
+            } else if constexpr (VEC) {
+                unsigned* to = (unsigned*)&image[kv_k_byte(a.dim64, t, d)];
+#pragma unroll
+                for (int w = 0; w < W; w += 4)
+                    to[w / 4] = __builtin_amdgcn_perm(b[w + 1], b[w], 0x0c0c0400u) | __builtin_amdgcn_perm(b[w + 3], b[w + 2], 0x04000c0cu);
+            } else {
+                image[kv_k_byte(a.dim64, t, d)] = (int8_t)b[0];
+            }
+        }
+    }
+    __syncthreads();
     auto again = [&](unsigned b) -> unsigned { return (unsigned)(int)rintf((float)(int8_t)b * ratio) & 255u; };
     const int w0 = grown ? 0 : t0;   // tokens whose codes change
     if (keys) {
@@ -300,17 +349,15 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs A) {
             const int t = tt * 16 + (u & 15), d0 = (c - tt * dc) * 64 + ((u >> 4) & 3) * 16;
             if (t < w0 || t >= t1 || d0 >= a.dim) continue;
             uint4* p = (uint4*)(dst + (int64_t)u * 16);
-            unsigned w[4] = {0, 0, 0, 0};
-            if (t < t0) {
-                const uint4 old = *p;
-                const unsigned ow[4] = {old.x, old.y, old.z, old.w};
-#pragma unroll
-                for (int j = 0; j < 16; j++) w[j >> 2] |= again(ow[j >> 2] >> (8 * (j & 3))) << (8 * (j & 3));
-            } else {
-#pragma unroll
-                for (int j = 0; j < 16; j++)
-                    if (VEC || d0 + j < a.dim) w[j >> 2] |= code(t, min(d0 + j, a.dim - 1)) << (8 * (j & 3));
+            if (t >= t0) {
+                *p = ((const uint4*)image)[u];
+                continue;
             }
+            const uint4 old = *p;
+            const unsigned ow[4] = {old.x, old.y, old.z, old.w};
+            unsigned w[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < 16; j++) w[j >> 2] |= again(ow[j >> 2] >> (8 * (j & 3))) << (8 * (j & 3));
             *p = make_uint4(w[0], w[1], w[2], w[3]);
         }
         return;
@@ -318,33 +365,22 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs A) {
     int8_t* dst = a.v + bi * (SMX_KV_BLOCK * (int64_t)a.dim64);
     if (t0 == 0 && t1 == SMX_KV_BLOCK) {
         // units of 8 tokens of channels d and d + 16, in memory order: (d / 32, token / 4 % 4, d % 16)
-        for (int u = tid; u < 2 * a.dim64; u += 256) {
-            const int d = (u >> 6) * 32 + (u & 15), t = ((u >> 4) & 3) * 4;
-            unsigned w[4] = {0, 0, 0, 0};
-#pragma unroll
-            for (int j = 0; j < 16; j++) {   // (d + 16 of an odd size may be past the head: any code)
-                const int dd = min(d + (j >> 3) * 16, a.dim - 1), tk = t + (j & 3) + ((j >> 2) & 1) * 16;
-                w[j >> 2] |= code(tk, dd) << (8 * (j & 3));
-            }
-            if (d < a.dim) *(uint4*)(dst + (int64_t)u * 16) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
+        for (int u = tid; u < 2 * a.dim64; u += 256)
+            if ((u >> 6) * 32 + (u & 15) < a.dim) *(uint4*)(dst + (int64_t)u * 16) = ((const uint4*)image)[u];
         return;
     }
     const int g0 = w0 >> 2, quads = ((t1 + 3) >> 2) - g0;   // groups of 4 tokens of a channel
     for (int it = tid; it < quads * a.dim; it += 256) {
-        const int q = it / a.dim, t = (g0 + q) * 4, d = it - q * a.dim;
-        int8_t* p = dst + kv_v_byte(t, d);
+        const int q = it / a.dim, t = (g0 + q) * 4, d = it - q * a.dim, at = kv_v_byte(t, d);
+        int8_t* p = dst + at;
         if (!grown && (t < t0 || t + 4 > t1)) {
-            for (int j = max(t0 - t, 0); j < min(t1 - t, 4); j++) p[j] = (int8_t)code(t + j, d);
+            for (int j = max(t0 - t, 0); j < min(t1 - t, 4); j++) p[j] = image[at + j];
             continue;
         }
-        unsigned w = 0;
-        const unsigned old = t < t0 ? *(const unsigned*)p : 0u;
-        for (int j = 0; j < 4; j++) {
-            unsigned b = 0;
-            if (t + j < t0) b = again(old >> (8 * j));
-            else if (t + j < t1) b = code(t + j, d);
-            w |= b << (8 * j);
+        unsigned w = *(const unsigned*)&image[at];   // (0 for tokens outside [t0, t1))
+        if (t < t0) {
+            const unsigned old = *(const unsigned*)p;
+            for (int j = 0; j < min(t0 - t, 4); j++) w |= again(old >> (8 * j)) << (8 * j);
         }
         *(unsigned*)p = w;
     }
@@ -352,7 +388,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs A) {
 
 // Workgroup (x, head, keys | values): the stored values of one block's rows.  A thread takes 4 tokens of 4 channels, four words of
 // the layout (a token's channels of keys, a channel's tokens of values), so that a wave's stores are whole pieces of rows: the
-// values are four times the bytes of the codes, and 16-byte stores to 64 rows at once took 26 us for 34 MB, these 12.
+// values are four times the bytes of the codes, and 16-byte stores to 64 rows at once took 26 us for 34 MB, these 9.5.
 template <bool VEC>
 __global__ __launch_bounds__(256) void kv_read_kernel(const KvArgs a, float* __restrict__ k, float* __restrict__ v) {
     const bool keys = blockIdx.z == 0;
@@ -466,7 +502,7 @@ int smx_kv_append_dev(smx_ctx* c, const smx_kv_cache* cache, const smx_kv_batch*
     if (batch->rows * q_heads >= (size_t(1) << 31) || A.touched + extra > INT_MAX)
         return fail(c, SMX_ERR_LIMIT, "kv_append_dev: %zu rows of %zu query heads", batch->rows, q_heads);
     const dim3 grid((unsigned)(A.touched + extra), (unsigned)cache->kv_heads, 2);
-    const size_t lds = SMX_KV_BLOCK * (cache->head_dim + 4) * 4;
+    const size_t lds = SMX_KV_BLOCK * (size_t)A.kv.dim64;
     ProfScope ps(c, "kv_append");
     auto pick = [&](auto bf16, auto two) {
         return vec ? kv_append_kernel<decltype(bf16)::value, decltype(two)::value, true> : kv_append_kernel<decltype(bf16)::value, decltype(two)::value, false>;
