@@ -12,7 +12,7 @@
 //   4  one workgroup for each row sorts the list (up to kList tokens), which places the cut at one token, finds the chunk that
 //      the pick falls into from the totals and the pick in the chunk
 // A row is read three times (without top_k and top_p: twice), every other launch from its end, where the one in front has left
-// the caches.  256 rows of 262144 (268 MB) with top_p: 52 + 66 + 63 + 11 us; one row with top_k and top_p:
+// the caches.  256 rows of 262144 (268 MB) with top_p on 3 rows of 4: 52 + 53 + 53 + 12 us; one row with top_k and top_p:
 // 4 + 8 + 4 + 4.  A list that does not fit (thousands of equal logits at the cut, or a cut more than kReach below the largest logit)
 // is found by bisection over the logits instead.
 #include <algorithm>
@@ -27,6 +27,7 @@ namespace smx {
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;    // of the row's own workgroup (launch 4)
+constexpr int kPartThreads = 512, kPartWaves = kPartThreads / 64;   // of a part's (launches 1 to 3)
 constexpr int kChunk = 1024;                             // tokens whose kept weight is totalled together
 constexpr int kMaxVocab = SMX_SAMPLE_MAX_VOCAB;   // (its chunks' totals are held in LDS)
 constexpr int kBins = 2048;
@@ -194,16 +195,34 @@ __device__ __forceinline__ void load_chunk(const Row& r, int chunk, float (&v)[1
     }
 }
 
+// Which part of which row a workgroup of launches 1 to 3 serves.  Workgroups go to the 8 XCDs in turn, so the same part is the same XCD's
+// in every launch (calls of up to a few tens of MB find their logits in its L2), from the end too (`back`: for larger ones, whose last
+// parts are still in the memory-side cache); and rows change places in groups of 8, so that rows that ask for alike work and recur with
+// a period of 2, 4 or 8 are not all one XCD's.
+struct Place {
+    int row, part;
+};
+__device__ __forceinline__ Place place_of(const SampleArgs& A, bool back) {
+    int id = blockIdx.y * A.parts + blockIdx.x;
+    if (back) {
+        const int whole = A.rows * A.parts & ~7;
+        if (id < whole) id = (whole - 8 - (id & ~7)) | (id & 7);
+    }
+    const int y = id / A.parts;
+    return Place{(y | 7) < A.rows ? (y & ~7) | ((y + (y >> 3)) & 7) : y, id - y * A.parts};
+}
+
 // Launch 1.  Workgroup (part, row); also clears what launches 2 and 3 add to.
-__global__ __launch_bounds__(1024) void sample_best_kernel(const SampleArgs A) {
-    __shared__ unsigned long long red[16];
-    const int row = blockIdx.y, part = blockIdx.x, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+__global__ __launch_bounds__(kPartThreads) void sample_best_kernel(const SampleArgs A) {
+    __shared__ unsigned long long red[kPartWaves];
+    const Place at = place_of(A, false);
+    const int row = at.row, part = at.part, wave = threadIdx.x >> 6;
     const Row x = row_of(A, row);
-    for (int i = part * blockDim.x + threadIdx.x; i < kBins; i += A.parts * blockDim.x) A.hist[(int64_t)row * kBins + i] = 0;
+    for (int i = part * kPartThreads + threadIdx.x; i < kBins; i += A.parts * kPartThreads) A.hist[(int64_t)row * kBins + i] = 0;
     if (part == 0 && threadIdx.x == 0) { A.cuts[row].done = 0; A.cuts[row].listed = 0; }
     unsigned bk = 0, bi = 0;
     const int c1 = min((part + 1) * A.part_chunks, A.chunks);
-    for (int c = part * A.part_chunks + wave; c < c1; c += waves) {
+    for (int c = part * A.part_chunks + wave; c < c1; c += kPartWaves) {
         float v[16];
         load_chunk(x, c, v);
         const int first = first_of(x, c);
@@ -217,7 +236,7 @@ __global__ __launch_bounds__(1024) void sample_best_kernel(const SampleArgs A) {
     if ((threadIdx.x & 63) == 0) red[wave] = b;
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int w = 1; w < waves; w++) b = max(b, red[w]);
+        for (int w = 1; w < kPartWaves; w++) b = max(b, red[w]);
         A.best[(int64_t)row * A.parts + part] = b;
     }
 }
@@ -240,19 +259,20 @@ __device__ __forceinline__ float floor_of_bin(const Ask& q, int bin) {
 }
 
 // Launch 2.  Workgroup (part, row), from the last to the first.  The last one of a row to finish reads the whole histogram: the
-// cut's bin is the first whose running total reaches top_k tokens, or floor(top_p * all weight).  256 rows of 262144: 66 us, 50 of
-// them the reading, 10 the LDS atomics.
-__global__ __launch_bounds__(1024) void sample_hist_kernel(const SampleArgs A) {
-    __shared__ unsigned long long hist[kBins], red[16];
+// cut's bin is the first whose running total reaches top_k tokens, or floor(top_p * all weight).  Bound by some 35 instructions a
+// token, the LDS atomic among them: 160 rows of 262144 with top_p and 96 without 53 us.
+__global__ __launch_bounds__(kPartThreads) void sample_hist_kernel(const SampleArgs A) {
+    __shared__ unsigned long long hist[kBins], red[kPartWaves];
     __shared__ unsigned done;
-    const int row = A.rows - 1 - blockIdx.y, part = A.parts - 1 - blockIdx.x, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    const Place at = place_of(A, true);
+    const int row = at.row, part = at.part, wave = threadIdx.x >> 6;
     const Ask q = ask_of(A, row);
     if (q.mode != kTopK && q.mode != kTopP) return;
     const Row x = row_of(A, row);
-    for (int i = threadIdx.x; i < kBins; i += blockDim.x) hist[i] = 0;
+    for (int i = threadIdx.x; i < kBins; i += kPartThreads) hist[i] = 0;
     __syncthreads();
     const int c0 = part * A.part_chunks, c1 = min(c0 + A.part_chunks, A.chunks);
-    for (int c = c1 - 1 - wave; c >= c0; c -= waves) {
+    for (int c = c1 - 1 - wave; c >= c0; c -= kPartWaves) {
         float v[16];
         load_chunk(x, c, v);
 #pragma unroll
@@ -265,33 +285,33 @@ __global__ __launch_bounds__(1024) void sample_hist_kernel(const SampleArgs A) {
     __syncthreads();
     unsigned long long* all = A.hist + (int64_t)row * kBins;
     RowCut* cut = A.cuts + row;
-    for (int i = threadIdx.x; i < kBins; i += blockDim.x) {
+    for (int i = threadIdx.x; i < kBins; i += kPartThreads) {
         const unsigned long long w = hist[i];
         if (w) atomicAdd(&all[i], w);
     }
     // What passes between workgroups is atomic at device scope, performed where all XCDs see it: this thread's additions are
     // waited for, then the workgroup counts itself; the reads below are atomic too.  (A fence by each wave would write its XCD's L2
-    // back: 256 rows of 262144 329 us instead of 66.)
+    // back: 256 rows of 262144 329 us instead of 75.)
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (threadIdx.x == 0) done = atomicAdd(&cut->done, 1u);
     __syncthreads();
     if (done != (unsigned)A.parts - 1) return;
-    const int per = kBins / blockDim.x;   // neighbouring bins for each thread: 2 or 4
-    unsigned long long bins[4], sum = 0;
+    constexpr int PER = kBins / kPartThreads;   // neighbouring bins for each thread
+    unsigned long long bins[PER], sum = 0;
 #pragma unroll
-    for (int j = 0; j < 4; j++)   // (all in flight at once)
-        bins[j] = j < per ? __hip_atomic_load(&all[threadIdx.x * per + j], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+    for (int j = 0; j < PER; j++)   // (all in flight at once)
+        bins[j] = __hip_atomic_load(&all[threadIdx.x * PER + j], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-        if (j < per) hist[threadIdx.x * per + j] = bins[j];
+    for (int j = 0; j < PER; j++) {
+        hist[threadIdx.x * PER + j] = bins[j];
         sum += bins[j];
     }
     unsigned long long run = wave_scan(sum);
     if ((threadIdx.x & 63) == 63) red[wave] = run;
     __syncthreads();
     unsigned long long total = 0, front = 0;
-    for (int w = 0; w < waves; w++) {
+    for (int w = 0; w < kPartWaves; w++) {
         if (w < wave) front += red[w];
         total += red[w];
     }
@@ -303,7 +323,7 @@ __global__ __launch_bounds__(1024) void sample_hist_kernel(const SampleArgs A) {
     if (threadIdx.x == 0) { bin = limit == 0 ? 0 : kBins; above = limit == 0 ? 0 : total; }
     __syncthreads();
     if (run < limit && run + sum >= limit) {
-        int i = threadIdx.x * per;
+        int i = threadIdx.x * PER;
         while (run + hist[i] < limit) run += hist[i++];
         bin = i;
         above = run;
@@ -317,12 +337,13 @@ __global__ __launch_bounds__(1024) void sample_hist_kernel(const SampleArgs A) {
 }
 
 // Launch 3.  Workgroup (part, row).  Tokens below the cut's bin take one comparison, the ones above it an exponential, the bin's own
-// (few) an LDS atomic.  256 rows of 262144 with top_p: 63 us, of which 45 are the reading; with the scalar registers for one
-// workgroup a CU (no second bound) 83.
-__global__ __launch_bounds__(1024, 8) void sample_gather_kernel(const SampleArgs A) {
+// (few) an LDS atomic.  256 rows of 262144, 224 of them to be read (235 MB), 160 with top_p: 53 us.  Its scalar registers are kept to what lets
+// 8 waves share a SIMD (7, and so a workgroup less on each CU, took 83 us where this took 63).
+__global__ __launch_bounds__(kPartThreads, 8) void sample_gather_kernel(const SampleArgs A) {
     __shared__ unsigned long long list[kList];
     __shared__ unsigned found, start;
-    const int row = blockIdx.y, part = blockIdx.x, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, lane = threadIdx.x & 63;
+    const Place at = place_of(A, false);
+    const int row = at.row, part = at.part, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const Ask q = ask_of(A, row);
     if (q.mode <= kGreedy) return;
     if (threadIdx.x == 0) found = 0;
@@ -332,7 +353,7 @@ __global__ __launch_bounds__(1024, 8) void sample_gather_kernel(const SampleArgs
     const float list_from = q.mode == kFree ? total_from : A.cuts[row].list_from;
     const Row x = row_of(A, row);
     const int c1 = min((part + 1) * A.part_chunks, A.chunks);
-    for (int c = part * A.part_chunks + wave; c < c1; c += waves) {
+    for (int c = part * A.part_chunks + wave; c < c1; c += kPartWaves) {
         float v[16];
         load_chunk(x, c, v);
         const int first = first_of(x, c);
@@ -360,7 +381,7 @@ __global__ __launch_bounds__(1024, 8) void sample_gather_kernel(const SampleArgs
     if (n == 0) return;
     if (threadIdx.x == 0) start = atomicAdd(&A.cuts[row].listed, n);
     __syncthreads();
-    for (unsigned i = threadIdx.x; i < n && start + i < (unsigned)kList; i += blockDim.x) A.list[(int64_t)row * kList + start + i] = list[i];
+    for (unsigned i = threadIdx.x; i < n && start + i < (unsigned)kList; i += kPartThreads) A.list[(int64_t)row * kList + start + i] = list[i];
 }
 
 struct Reduce {
@@ -801,12 +822,13 @@ int launch_sample(smx_ctx* c, const float* logits, size_t rows, size_t vocab, si
     A.chunks = (int)((vocab + skew + kChunk - 1) / kChunk);
     if (p) { A.temperature = p->temperature; A.top_k = p->top_k; A.top_p = p->top_p; A.min_p = p->min_p; }
     A.u = u; A.ids = ids; A.prob = prob;
-    // Parts of a row: 512 workgroups in all (two a CU), of at least one chunk a wave.  Workgroups of 8 waves where a call is small: more
-    // of them for a row, though each adds a histogram to the row's; of 16 where there is work for all of them anyhow.  4 / 8 / 16 waves,
-    // us of the four launches with top_p: 1 x 131072 26.4 / 26.0 / 28.3, 16 x 131072 34.0 / 30.7 / 33.4, 32 x 131072
-    // 42.8 / 37.9 / 38.3, 64 x 131072 55.6 / 48.2 / 46.6, 64 x 32000 31.7 / 29.2 / 31.7.
-    const int threads = rows * (size_t)A.chunks < 4096 ? 512 : 1024;
-    const size_t waves = threads / 64, want = 512, most = ((size_t)A.chunks + waves - 1) / waves;
+    // Parts of a row: workgroups of 8 waves, of at least one chunk a wave.  More of them balance rows that ask for different work (greedy
+    // ones end at once), but each adds a histogram to its row's.  512 / 1024 / 2048 in all, us of the four launches, rows that ask for
+    // different things and, behind them, alike: 20 x 262144 41.6 / 41.5 / 41.8 and 43 / 43 / 43, 40 x 262144 57 / 57 / 58 and
+    // 56 / 63 / 62, 64 x 262144 70 / 66 / 73 and 70 / 67 / 78, 256 x 262144 203 / 185 / 170 and 198 / 180 / 182,
+    // 1000 x 50000 226 / 167 / 159 and 215 / 162 / 175.
+    const size_t all = rows * (size_t)A.chunks, waves = kPartWaves, most = ((size_t)A.chunks + waves - 1) / waves;
+    const size_t want = all >= 2048 * 32 ? 2048 : all >= 1024 * 12 ? 1024 : 512;
     size_t parts = std::max<size_t>(1, std::min(most, (want + rows - 1) / rows));
     // whole rounds of the waves
     A.part_chunks = (int)std::max<size_t>(waves, ((A.chunks + parts - 1) / parts + waves / 2) / waves * waves);
@@ -839,9 +861,9 @@ int launch_sample(smx_ctx* c, const float* logits, size_t rows, size_t vocab, si
         G.u += r; G.ids += r;
         if (prob) G.prob += r;
         const dim3 grid((unsigned)A.parts, (unsigned)n);
-        hipLaunchKernelGGL(sample_best_kernel, grid, dim3(threads), 0, c->stream, G);
-        if (cuts) hipLaunchKernelGGL(sample_hist_kernel, grid, dim3(threads), 0, c->stream, G);
-        hipLaunchKernelGGL(sample_gather_kernel, grid, dim3(threads), 0, c->stream, G);
+        hipLaunchKernelGGL(sample_best_kernel, grid, dim3(kPartThreads), 0, c->stream, G);
+        if (cuts) hipLaunchKernelGGL(sample_hist_kernel, grid, dim3(kPartThreads), 0, c->stream, G);
+        hipLaunchKernelGGL(sample_gather_kernel, grid, dim3(kPartThreads), 0, c->stream, G);
         hipLaunchKernelGGL(sample_pick_kernel, dim3((unsigned)n), dim3(kThreads), lds, c->stream, G);
         SMX_HIP(c, hipGetLastError());
     }
