@@ -327,10 +327,22 @@ int launch_tile(smx_ctx* c, const AttnArgs& A, dim3 grid) {
     return SMX_OK;
 }
 // Column tiles of a wave: as many as leave two waves a SIMD their registers (queries and sums are 8 CT DC NT and 16 CT DC of 256).
-constexpr int wave_tiles(int dc) { return dc <= 2 ? 2 : 1; }
+// Column tiles of a wave: as many as leave two waves a SIMD their registers (queries and sums are 8 CT DC NT and 16 CT DC of 256).
+constexpr int most_wave_tiles(int dc) { return dc <= 2 ? 2 : 1; }
+// Rows of a workgroup in units of 64: 128 (they share each widened byte), or 64 where the work does not fill the chip for long, which makes
+// more workgroups with a shorter way each.  The measure is pairs of a row and a key for each CU; f32 rows of 65..128 channels stay with 64
+// for longer, since 128 of them spill some registers.  us at 64 / 128 rows, 32 heads over 8 key/value heads of 128 channels, bf16 and f32:
+// 32 tokens behind 4000 21 / 29 and 23 / 32, 40 tokens of 4 sequences of 4000 45 / 44 and 54 / 66, 96 of 4 of 16000 249 / 168 and
+// 312 / 261, 512 of 4 of 16000 907 / 649 and 1164 / 1074.
+int tile_waves(const smx_ctx* c, const AttnArgs& A, size_t rows, size_t reach, bool bf16) {
+    const int dc = A.kv.dim64 / 64;
+    const double pairs = (double)A.kv.nseq * A.kv.kv_heads * (double)rows * (double)reach / c->num_cu;
+    return pairs < (dc == 2 && !bf16 ? 4e5 : 1e5) ? 1 : most_wave_tiles(dc);
+}
 template <int DC>
 int launch_dim(smx_ctx* c, const AttnArgs& A, dim3 grid, bool bf16) {
-    return bf16 ? launch_tile<DC, wave_tiles(DC), 1, true>(c, A, grid) : launch_tile<DC, wave_tiles(DC), 2, false>(c, A, grid);
+    if (A.tile_rows == 64) return bf16 ? launch_tile<DC, 1, 1, true>(c, A, grid) : launch_tile<DC, 1, 2, false>(c, A, grid);
+    return bf16 ? launch_tile<DC, most_wave_tiles(DC), 1, true>(c, A, grid) : launch_tile<DC, most_wave_tiles(DC), 2, false>(c, A, grid);
 }
 
 }  // namespace
@@ -371,7 +383,7 @@ extern "C" int smx_attn_dev(smx_ctx* c, const smx_kv_cache* cache, const smx_kv_
     // tokens in reach of one sequence's rows
     const size_t reach = window ? std::min<size_t>(A.kv.max_len, window + batch->max_rows + SMX_KV_BLOCK) : (size_t)A.kv.max_len;
     const bool few = tile_rows <= 64;
-    A.tile_rows = few ? rows_per_tile(A.kv.dim64, tile_rows) : 64 * wave_tiles(dc);
+    A.tile_rows = few ? rows_per_tile(A.kv.dim64, tile_rows) : 64 * tile_waves(c, A, tile_rows, reach, bf16);
     A.row_tiles = (int)((tile_rows + A.tile_rows - 1) / A.tile_rows);
     // how many workgroups the sequences make without a split
     const size_t groups = batch->nseq * cache->kv_heads * (size_t)A.row_tiles;
