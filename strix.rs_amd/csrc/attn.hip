@@ -263,6 +263,46 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(const AttnArgs A) {
     }
 }
 
+// The sequence of a row.
+__device__ __forceinline__ int seq_of_row(const KvArgs& a, int row) {
+    if (!a.row0) return row;
+    int lo = 0, hi = a.nseq - 1;   // the last one that starts at or before the row
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (a.row0[mid] <= row) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+}
+
+// Up to kJoinFew pieces: dim64 / 4 threads for a (row, head), each with 4 channels of every piece.  A workgroup for each (row, head) as
+// below / this: 96 rows of 16 sequences in 2 pieces 47 / 34 us with the attention, 24 rows of 4 in 7 pieces 25 / 21; more pieces than that
+// (64 for one row) 58 / 64.
+constexpr int kJoinFew = 16;
+template <bool BF16>
+__global__ __launch_bounds__(256) void attn_join_few_kernel(const AttnArgs A) {
+    const int quads = A.kv.dim64 >> 2, nth = threadIdx.x / quads, units = 256 / quads, d = (threadIdx.x - nth * quads) * 4;   // quads: 16, 32, 48 or 64
+    const int unit = blockIdx.x * units + nth, row = unit / A.q_heads, head = unit - row * A.q_heads;
+    if (nth >= units || row >= A.kv.rows) return;
+    const Span sp = seq_span(A, seq_of_row(A.kv, row));
+    if (sp.pieces <= 1 || row >= sp.q.row + sp.q.n) return;
+    const int64_t at = (int64_t)unit * A.pieces;
+    float M = kNoMax, L = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < sp.pieces; i++) M = fmaxf(M, A.part_ml[at + i].x);
+    v4f acc = v4f{0.f, 0.f, 0.f, 0.f};
+    const float* from = A.part + at * A.kv.dim64 + d;
+#pragma unroll 4
+    for (int i = 0; i < sp.pieces; i++) {
+        const float2 ml = A.part_ml[at + i];
+        const float f = ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - M);   // (a piece without a key for the row)
+        acc += *(const v4f*)(from + (int64_t)i * A.kv.dim64) * f;
+        L += ml.y * f;
+    }
+    RowAt r;
+    r.row = row; r.head = head; r.pos = 0; r.live = true;
+    store_out<BF16>(A, r, d, acc * (L > 0.f ? 1.0f / L : L == L ? 0.f : L));
+}
+
 // Workgroup (row, head): the pieces of a long sequence joined.  Every piece's factor is formed first, so that nothing stands between
 // the loads of their sums; 16 bytes for each thread, several pieces at a time.
 template <bool BF16>
@@ -270,16 +310,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs A) {
     __shared__ float factor[kMaxPieces], red[2][4];
     __shared__ v4f sums[256];
     const int row = blockIdx.x, head = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    int s = row;
-    if (A.kv.row0) {
-        int lo = 0, hi = A.kv.nseq - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (A.kv.row0[mid] <= row) lo = mid; else hi = mid - 1;
-        }
-        s = lo;
-    }
-    const Span sp = seq_span(A, s);
+    const Span sp = seq_span(A, seq_of_row(A.kv, row));
     if (sp.pieces <= 1 || row >= sp.q.row + sp.q.n) return;
     const int64_t at = ((int64_t)row * A.q_heads + head) * A.pieces;
     float M = kNoMax;
@@ -356,6 +387,9 @@ using namespace smx;
 // (1408 / 640); 72 rows, 20 of 16000 174 / 120.  Many rows (40 tokens of 32 heads of 128 channels, 8 key/value heads): 1 of 4000
 // 27.8 / 31.0 (256 / 128), 1 of 16000 47 / 40 (1024 / 512), 4 of 4000 52 / 45 (1024 / 512).
 constexpr size_t kWorthFew = 512, kWorthMany = 256;
+// Contexts that are not split at all: the join costs more than it shortens.  Whole / in pieces of 128 tokens, 4 sequences: one row of 200
+// tokens 8.8 / 10.2, of 350 9.8 / 10.3, of 600 11.8 / 11.4; 64 rows of 200 15.6 / 22.3, of 350 19.7 / 22.7, of 600 26.4 / 26.1.
+constexpr size_t kWhole = 384;
 
 extern "C" int smx_attn_dev(smx_ctx* c, const smx_kv_cache* cache, const smx_kv_batch* batch, int type, const void* q, size_t ldq, size_t q_heads,
                             float scale, size_t window, void* out, size_t ldo) {
@@ -390,7 +424,8 @@ extern "C" int smx_attn_dev(smx_ctx* c, const smx_kv_cache* cache, const smx_kv_
     // one to a CU, or two where that leaves each enough tokens; never a few more than that, which would wait for a round of their own
     const size_t cus = c->num_cu, span = std::max<size_t>(reach, 1);
     size_t split = std::max<size_t>(1, cus / groups);
-    if (2 * cus / groups > split && span / (2 * cus / groups) >= (few ? kWorthFew : kWorthMany)) split = 2 * cus / groups;
+    if (span <= kWhole) split = 1;
+    else if (2 * cus / groups > split && span / (2 * cus / groups) >= (few ? kWorthFew : kWorthMany)) split = 2 * cus / groups;
     split = std::min<size_t>(split, kMaxPieces);
     const size_t piece = std::max<size_t>(((span + split - 1) / split + 127) & ~size_t(127), 128);
     A.piece = (int)std::min<size_t>(piece, size_t(1) << 30);
@@ -418,9 +453,16 @@ extern "C" int smx_attn_dev(smx_ctx* c, const smx_kv_cache* cache, const smx_kv_
     SMX_HIP(c, hipGetLastError());
     if (A.pieces > 1 && !A.join) {
         ProfScope ps(c, "attn_join");
-        const dim3 jg((unsigned)batch->rows, (unsigned)q_heads);
-        if (bf16) hipLaunchKernelGGL(attn_join_kernel<true>, jg, dim3(256), 0, c->stream, A);
-        else hipLaunchKernelGGL(attn_join_kernel<false>, jg, dim3(256), 0, c->stream, A);
+        if (A.pieces <= kJoinFew) {
+            const size_t units = 256 / (A.kv.dim64 / 4);
+            const dim3 jg((unsigned)((batch->rows * q_heads + units - 1) / units));
+            if (bf16) hipLaunchKernelGGL(attn_join_few_kernel<true>, jg, dim3(256), 0, c->stream, A);
+            else hipLaunchKernelGGL(attn_join_few_kernel<false>, jg, dim3(256), 0, c->stream, A);
+        } else {
+            const dim3 jg((unsigned)batch->rows, (unsigned)q_heads);
+            if (bf16) hipLaunchKernelGGL(attn_join_kernel<true>, jg, dim3(256), 0, c->stream, A);
+            else hipLaunchKernelGGL(attn_join_kernel<false>, jg, dim3(256), 0, c->stream, A);
+        }
         SMX_HIP(c, hipGetLastError());
     }
     return SMX_OK;
