@@ -13,8 +13,8 @@
 //      the pick falls into from the totals and the pick in the chunk
 // A row is read three times (without top_k and top_p: twice), every other launch from its end, where the one in front has left
 // the caches.  256 rows of 262144 (268 MB) with top_p on 3 rows of 4: 52 + 53 + 53 + 12 us; one row with top_k and top_p:
-// 4 + 8 + 4 + 4.  A list that does not fit (thousands of equal logits at the cut, or a cut more than kReach below the largest logit)
-// is found by bisection over the logits instead.
+// 4 + 8 + 4 + 4.  A list that does not fit (top_k of thousands, thousands of equal logits at the cut, or a cut more than kReach below
+// the largest logit) is done without: the row's own workgroup looks for the cut in steps of the logits' keys.
 #include <algorithm>
 #include <climits>
 #include <cmath>
@@ -34,7 +34,6 @@ constexpr int kBins = 2048;
 constexpr float kReach = 28.0f;                          // exp(-28) < 2^-40: beyond it there is no weight
 constexpr int kList = 4096;
 constexpr int kSteps = 1024;                             // of a long list's keys
-constexpr int kWays = 7;                                 // keys that a step of the bisection tries
 
 struct SampleArgs {
     const float* logits;
@@ -563,90 +562,114 @@ __device__ Last place(const SampleArgs& A, const Ask& q, Reduce& red, const unsi
     return Last{~(unsigned)(best >> 32), (unsigned)best};
 }
 
-// The cut of a row whose list overflowed, by bisection over the keys and then over the indices of the key's tokens.
-__device__ Last cut_by_bisection(const SampleArgs& A, const Ask& q, int row, Reduce& red) {
-    const float* x = A.logits + (int64_t)row * A.ld;
-    const int V = A.vocab;
-    // tokens, or weight, of keys > k for kWays keys k at once
-    auto above = [&](const unsigned (&k)[kWays], bool weighed, unsigned long long (&t)[kWays]) {
-#pragma unroll
-        for (int w = 0; w < kWays; w++) t[w] = 0;
-        for (int i = threadIdx.x; i < V; i += kThreads) {
-            const float v = x[i];
-            const unsigned key = key_of(v);
-            if (key <= k[0]) continue;
-            const unsigned long long m = weighed ? weight(q.share(v)) : 1ull;
-#pragma unroll
-            for (int w = 0; w < kWays; w++) t[w] += key > k[w] ? m : 0ull;
+// f(logit, index) for every token of a lane's share of a chunk, 4 at a time (a row's own workgroup has other uses for registers).
+template <class F>
+__device__ __forceinline__ void each_token(const Row& r, int chunk, F&& f) {
+    const int first = first_of(r, chunk);
+#pragma unroll 1
+    for (int j = 0; j < 4; j++) {
+        const int i = first + 256 * j;
+        float4 v = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        if (i >= 0 && i + 4 <= r.vocab) {
+            v = *(const float4*)(r.x + i);
+        } else {
+            if (i >= 0 && i < r.vocab) v.x = r.x[i];
+            if (i + 1 >= 0 && i + 1 < r.vocab) v.y = r.x[i + 1];
+            if (i + 2 >= 0 && i + 2 < r.vocab) v.z = r.x[i + 2];
+            if (i + 3 >= 0 && i + 3 < r.vocab) v.w = r.x[i + 3];
         }
-#pragma unroll
-        for (int w = 0; w < kWays; w++) t[w] = block_sum(red, t[w]);
-    };
-    auto one_above = [&](unsigned k, bool weighed) {
-        unsigned ks[kWays];
-        unsigned long long t[kWays];
-#pragma unroll
-        for (int w = 0; w < kWays; w++) ks[w] = k;
-        above(ks, weighed, t);
-        return t[0];
-    };
-    // the smallest key in [lo, hi] with less than `limit` above it; hi has
-    auto smallest = [&](unsigned lo, unsigned hi, bool weighed, unsigned long long limit) {
-        while (lo < hi) {
-            const unsigned step = (hi - lo) / (kWays + 1) + 1;
-            unsigned ks[kWays];
-            unsigned long long t[kWays];
-#pragma unroll
-            for (int w = 0; w < kWays; w++) ks[w] = hi - lo > (unsigned)w * step ? lo + (unsigned)w * step : hi;
-            above(ks, weighed, t);
-            unsigned nlo = lo, nhi = hi;
-#pragma unroll
-            for (int w = kWays - 1; w >= 0; w--)
-                if (t[w] < limit) nhi = ks[w];
-#pragma unroll
-            for (int w = 0; w < kWays; w++)
-                if (!(t[w] < limit)) nlo = ks[w] + 1;
-            lo = nlo;
-            hi = nhi;
+        f(v.x, (unsigned)i);
+        f(v.y, (unsigned)i + 1);
+        f(v.z, (unsigned)i + 2);
+        f(v.w, (unsigned)i + 3);
+    }
+}
+
+// The cut of a row whose list overflowed, in steps of kBins ranges of keys (three at most) and then by the index among the last key's tokens.
+// bins [kBins], counts [chunks].  A row of 262144 with top_k = 20000 0.6 ms, with top_p in it 1.1 (bisection over the keys 5.0 and 9.3).
+__device__ Last cut_by_steps(const SampleArgs& A, const Ask& q, const Row& r, Reduce& red, unsigned long long* bins, unsigned long long* counts,
+                             unsigned long long* found) {
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const unsigned top = key_of(q.mx);
+    // index of the n-th (from 1) token of a key that the bound keeps
+    auto nth = [&](unsigned key, unsigned long long n, Last bound) {
+        for (int c = wave; c < A.chunks; c += kWaves) {
+            unsigned m = 0;
+            each_token(r, c, [&](float v, unsigned i) { m += key_of(v) == key && kept(bound, key, i); });
+            const unsigned long long t = wave_sum(m);
+            if (lane == 0) counts[c] = t;
         }
-        return lo;
-    };
-    // index of the n-th (from 1) token of key k, the last one if there are fewer
-    auto nth = [&](unsigned k, unsigned long long n) {
-        unsigned lo = 0, hi = (unsigned)V - 1;
-        while (lo < hi) {
-            const unsigned mid = lo + (hi - lo) / 2;
-            unsigned long long t = 0;
-            for (unsigned i = threadIdx.x; i <= mid; i += kThreads) t += key_of(x[i]) == k;
-            if (block_sum(red, t) >= n) hi = mid; else lo = mid + 1;
+        __syncthreads();
+        const int per = (A.chunks + kThreads - 1) / kThreads, c0 = min(tid * per, A.chunks), c1 = min(c0 + per, A.chunks);
+        unsigned long long sum = 0;
+        for (int c = c0; c < c1; c++) sum += counts[c];
+        unsigned long long run = block_scan(red, sum) - sum;
+        if (run < n && n <= run + sum) {
+            int c = c0;
+            while (run + counts[c] < n) run += counts[c++];
+            found[0] = c;
+            found[1] = n - run;
         }
-        return lo;
+        __syncthreads();
+        const int first = (int)found[0] * kChunk - r.skew + tid * (kChunk / kThreads);
+        const unsigned long long left = found[1];
+        sum = 0;
+        for (int e = 0; e < kChunk / kThreads; e++) sum += first + e >= 0 && first + e < r.vocab && key_of(r.x[first + e]) == key;
+        run = block_scan(red, sum) - sum;
+        if (run < left && left <= run + sum) {
+            int e = 0;
+            for (; run < left; e++) run += first + e >= 0 && first + e < r.vocab && key_of(r.x[first + e]) == key;
+            found[0] = first + e - 1;
+        }
+        __syncthreads();
+        return (unsigned)found[0];
+    };
+    // the last of the bound's tokens, in order, with less than the limit in front of it: `limit` tokens, or (weighed) top_p of their weight
+    auto cut = [&](Last bound, bool weighed, unsigned long long limit) {
+        unsigned lo = max(bound.key, 1u), hi = top;
+        unsigned long long front = 0;
+        for (bool whole = true;; whole = false) {
+            const int shift = max(0, 21 - __clz(hi - lo | 1));   // (hi - lo) >> shift < kBins
+            for (int i = tid; i < kBins; i += kThreads) bins[i] = 0;
+            if (tid == 0) found[0] = kBins;
+            __syncthreads();
+            for (int c = wave; c < A.chunks; c += kWaves)
+                each_token(r, c, [&](float v, unsigned i) {
+                    const unsigned k = key_of(v);
+                    if (k < lo || k > hi || !kept(bound, k, i)) return;
+                    const unsigned long long w = weighed ? weight(q.share(v)) : 1ull;
+                    if (w) atomicAdd(&bins[(hi - k) >> shift], w);
+                });
+            __syncthreads();
+            constexpr int PER = kBins / kThreads;
+            unsigned long long sum = 0;
+            for (int i = 0; i < PER; i++) sum += bins[tid * PER + i];
+            if (whole && weighed) {
+                limit = (unsigned long long)((double)q.top_p * (double)block_sum(red, sum));
+                if (limit == 0) return Last{top, q.best_at};
+            }
+            unsigned long long run = front + block_scan(red, sum) - sum;
+            if (run < limit && run + sum >= limit) {
+                int i = tid * PER;
+                while (run + bins[i] < limit) run += bins[i++];
+                found[0] = i;
+                found[1] = run;
+            }
+            __syncthreads();
+            const unsigned b = (unsigned)found[0];
+            if (b == kBins) return bound;   // everything fits
+            front = found[1];
+            hi -= b << shift;
+            lo = hi - min((1u << shift) - 1, hi - lo);
+            __syncthreads();
+            if (shift == 0) break;
+        }
+        const unsigned long long w = weighed ? weight(q.share(of_key(hi))) : 1ull;
+        return Last{hi, nth(hi, (limit - front + w - 1) / w, bound)};
     };
     Last l = {0u, 0xffffffffu};
-    unsigned long long ties = 0;   // kept tokens of key l.key
-    const unsigned top = key_of(q.mx);
-    if (q.mode == kTopK) {
-        unsigned lo = smallest(0u, top, false, (unsigned long long)q.top_k);   // fewer than top_k tokens above it
-        if (lo == 0) lo = 1;       // (fewer candidates than top_k: all of them)
-        const unsigned long long front = one_above(lo, false);
-        ties = min((unsigned long long)q.top_k - front, one_above(lo - 1, false) - front);
-        l.key = lo;
-        l.at = ties ? nth(lo, ties) : 0u;
-    }
-    if (q.top_p < 1.0f) {
-        const unsigned long long w_key = l.key ? weight(q.share(of_key(l.key))) : 0;
-        const unsigned long long total = one_above(l.key, true) + ties * w_key;
-        const unsigned long long limit = (unsigned long long)((double)q.top_p * (double)total);
-        if (limit == 0) return Last{top, q.best_at};
-        const unsigned lo = smallest(l.key, top, true, limit);
-        const unsigned long long w = lo ? weight(q.share(of_key(lo))) : 0;
-        const unsigned long long n = w ? (limit - one_above(lo, true) + w - 1) / w : 0;
-        if (lo != l.key || n < ties) {
-            l.key = lo;
-            l.at = n ? nth(lo, n) : 0u;
-        }
-    }
-    return l;
+    if (q.mode == kTopK) l = cut(l, false, (unsigned long long)q.top_k);
+    return q.top_p < 1.0f ? cut(l, true, 0) : l;
 }
 
 // Launch 4.  Workgroup: a row.
@@ -679,7 +702,7 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(const SampleArgs 
         fits = cut.listed <= (unsigned)kList;
         const int n = fits ? (int)cut.listed : 0;
         if (!fits) {
-            last = cut_by_bisection(A, q, row, red);
+            last = cut_by_steps(A, q, r, red, members, totals, found);
         } else if (n <= kThreads) {
             // a token for each thread; its rank and the weight in front of it by comparing with every other
             const unsigned long long mine = tid < n ? from[tid] : ~0ull;
@@ -751,16 +774,14 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(const SampleArgs 
     __syncthreads();
     if (!fits) {
         for (int c = tid >> 6; c < A.chunks; c += kWaves) {
-            unsigned long long t = 0;
-            for (int i = max(c * kChunk - r.skew, 0) + (tid & 63); i < min((c + 1) * kChunk - r.skew, A.vocab); i += 64) {
-                const float v = x[i];
-                if (v > -INFINITY && kept(last, key_of(v), (unsigned)i)) {
-                    const float e = q.share(v);
-                    if (e >= q.min_p) t += weight(e);
-                }
-            }
-            t = wave_sum(t);
-            if ((tid & 63) == 0) totals[c] = t;
+            double t = 0;   // of 16 whole numbers up to 2^40: exact
+            each_token(r, c, [&](float v, unsigned i) {
+                if (!(v > -INFINITY) || !kept(last, key_of(v), i)) return;
+                const float e = q.share(v);
+                if (e >= q.min_p) t += (double)truncf(e * 0x1p40f);
+            });
+            const unsigned long long total = wave_sum((unsigned long long)t);
+            if ((tid & 63) == 0) totals[c] = total;
         }
     } else {
         for (int i = tid; i < keep; i += kThreads) {   // the list's kept tokens (none without a cut)
