@@ -391,6 +391,11 @@ constexpr size_t kWorthFew = 512, kWorthMany = 256;
 // tokens 8.8 / 10.2, of 350 9.8 / 10.3, of 600 11.8 / 11.4; 64 rows of 200 15.6 / 22.3, of 350 19.7 / 22.7, of 600 26.4 / 26.1.
 constexpr size_t kWhole = 384;
 
+// Tokens of 128 channels of a piece, however many sequences there are: the call knows the longest only, and one long sequence among short ones
+// would keep a few workgroups busy for long after the others.  One row each of 64 sequences of 500 tokens and one of 131072: 145 us, without
+// 1163; 64 of 33..32768 430 / 462; where all are alike it costs a little: 64 of 16384 394 / 370.
+constexpr size_t kLongest = 8192, kMostSums = size_t(256) << 20;
+
 extern "C" int smx_attn_dev(smx_ctx* c, const smx_kv_cache* cache, const smx_kv_batch* batch, int type, const void* q, size_t ldq, size_t q_heads,
                             float scale, size_t window, void* out, size_t ldo) {
     if (!c) return SMX_ERR_ARG;
@@ -426,6 +431,9 @@ extern "C" int smx_attn_dev(smx_ctx* c, const smx_kv_cache* cache, const smx_kv_
     size_t split = std::max<size_t>(1, cus / groups);
     if (span <= kWhole) split = 1;
     else if (2 * cus / groups > split && span / (2 * cus / groups) >= (few ? kWorthFew : kWorthMany)) split = 2 * cus / groups;
+    // and no piece is longer than kLongest to 2 kLongest, as far as there is room for the pieces' sums
+    const size_t sums = batch->rows * q_heads * ((size_t)A.kv.dim64 * 4 + 8);
+    split = std::max(split, std::min<size_t>(span * A.kv.dim64 / 128 / kLongest, kMostSums / sums));
     split = std::min<size_t>(split, kMaxPieces);
     const size_t piece = std::max<size_t>(((span + split - 1) / split + 127) & ~size_t(127), 128);
     A.piece = (int)std::min<size_t>(piece, size_t(1) << 30);

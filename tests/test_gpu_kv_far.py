@@ -104,3 +104,27 @@ def test_splits_and_joins(accel, pkg, group, new):
                 assert np.abs(got - want).max() <= 2e-5 * np.abs(v).max(), (kv, lens, again)
                 first = got if again == 0 else first
             assert np.array_equal(first, got)   # (whichever workgroup joins the pieces, they are added in the same order)
+
+
+@pytest.mark.parametrize("new,ty", [(1, "f32"), (3, "f32"), (40, "bf16")])
+def test_one_long_sequence_among_many(accel, pkg, new, ty):
+    """A batch that fills the chip with short sequences, and a long one that is split all the same."""
+    rng = np.random.default_rng(33 + new)
+    kv, heads, dim, page = 8, 16, 128, 64
+    lens = [int(n) for n in rng.integers(new, 90, 63)] + [16500]
+    cache = R.Cache(sum(-(-n // page) for n in lens) + 1, page, kv, dim, seed=new)
+    cache.ks[:], cache.vs[:] = (rng.uniform(0.001, 0.02, cache.ks.shape).astype(np.float32) for _ in range(2))
+    table = R.tables(rng, cache.pages, page, lens)
+    n = [new] * len(lens)
+    q = rng.standard_normal((sum(n), heads, dim)).astype(np.float32)
+    raw = q if ty == "f32" else R.bf16(q)
+    q = q if ty == "f32" else R.from_bf16(raw)
+    want = R.attend(cache, table, lens, n, q, dim ** -0.5)
+    with R.Dev(accel) as dev:
+        d = R.OnDevice(pkg, dev, cache)
+        out = dev.room(raw.nbytes)
+        accel.attn_dev(d.handle, d.batch(table, lens, n), dev.put(raw), heads, dim ** -0.5, out, dtype=pkg.DTYPE_F32 if ty == "f32" else pkg.DTYPE_BF16)
+        got = dev.get(out, raw.shape, raw.dtype)
+    got = got if ty == "f32" else R.from_bf16(got)
+    # values of up to 128 * 0.02; the bounds that the tests of attention derive: 2e-5 of that, bf16 2^-8 of it
+    assert np.abs(got - want).max() <= (2e-5 if ty == "f32" else 2.0 ** -8) * 128 * 0.02
