@@ -8,6 +8,21 @@ namespace smx {
 
 namespace {
 
+// The n-th (from 0) of the sequences that are this launch's; -1: there are fewer.
+__device__ __forceinline__ int nth_sequence(const AttnArgs& A, int n) {
+    for (int base = 0; base < A.kv.nseq; base += 64) {   // a wave looks at 64 at a time
+        const int s = base + (threadIdx.x & 63);
+        unsigned long long hit = __ballot(s < A.kv.nseq && kv_seq(A.kv, s).n * (int64_t)A.group > A.above);
+        const int found = __popcll(hit);
+        if (n < found) {
+            for (; n > 0; n--) hit &= hit - 1;
+            return base + __ffsll((long long)hit) - 1;
+        }
+        n -= found;
+    }
+    return -1;
+}
+
 // ---- many rows: a prompt chunk.  Workgroup (head and tile of 64 CT rows, piece, sequence); a wave holds 16 CT rows, and the four
 // share tiles of TB blocks that are widened to f16 on their way into LDS (each byte once per workgroup), two of them in turn; the tile
 // behind the next one is in flight in registers.
@@ -20,7 +35,8 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(const AttnArgs A) {
     constexpr int KEYS = TB * 2 * KF * 64, TILE = KEYS + TB * NO * 64;   // 16-byte words: keys [block][token / 16][KF][lane], values [block][NO][lane]
     __shared__ Segment seg;
     extern __shared__ uint4 stage[];   // [2][TILE]
-    const int s = blockIdx.z, piece = blockIdx.y;
+    const int s = A.listed ? nth_sequence(A, blockIdx.z) : blockIdx.z, piece = blockIdx.y;
+    if (s < 0) return;
     const int kvh = blockIdx.x % A.kv.kv_heads;
     // The longest rows first.  Where every workgroup has a place at once (two on a CU), the second half goes the other way round, so that
     // each CU has a long and a short one.
@@ -365,9 +381,9 @@ constexpr int most_wave_tiles(int dc) { return dc <= 2 ? 2 : 1; }
 // for longer, since 128 of them spill some registers.  us at 64 / 128 rows, 32 heads over 8 key/value heads of 128 channels, bf16 and f32:
 // 32 tokens behind 4000 21 / 29 and 23 / 32, 40 tokens of 4 sequences of 4000 45 / 44 and 54 / 66, 96 of 4 of 16000 249 / 168 and
 // 312 / 261, 512 of 4 of 16000 907 / 649 and 1164 / 1074.
-int tile_waves(const smx_ctx* c, const AttnArgs& A, size_t rows, size_t reach, bool bf16) {
+int tile_waves(const smx_ctx* c, const AttnArgs& A, size_t nseq, size_t rows, size_t reach, bool bf16) {
     const int dc = A.kv.dim64 / 64;
-    const double pairs = (double)A.kv.nseq * A.kv.kv_heads * (double)rows * (double)reach / c->num_cu;
+    const double pairs = (double)nseq * A.kv.kv_heads * (double)rows * (double)reach / c->num_cu;
     return pairs < (dc == 2 && !bf16 ? 4e5 : 1e5) ? 1 : most_wave_tiles(dc);
 }
 template <int DC>
@@ -375,11 +391,6 @@ int launch_dim(smx_ctx* c, const AttnArgs& A, dim3 grid, bool bf16) {
     if (A.tile_rows == 64) return bf16 ? launch_tile<DC, 1, 1, true>(c, A, grid) : launch_tile<DC, 1, 2, false>(c, A, grid);
     return bf16 ? launch_tile<DC, most_wave_tiles(DC), 1, true>(c, A, grid) : launch_tile<DC, most_wave_tiles(DC), 2, false>(c, A, grid);
 }
-
-}  // namespace
-}  // namespace smx
-
-using namespace smx;
 
 // Tokens that are worth a second workgroup on a CU (a workgroup's start and its share of the join cost as much as some 200).  us at one
 // workgroup a CU / two, with the pieces' tokens.  Few rows (24 of 80 channels, 4 key/value heads): 1 sequence of 16000 tokens
@@ -395,6 +406,75 @@ constexpr size_t kWhole = 384;
 // would keep a few workgroups busy for long after the others.  One row each of 64 sequences of 500 tokens and one of 131072: 145 us, without
 // 1163; 64 of 33..32768 430 / 462; where all are alike it costs a little: 64 of 16384 394 / 370.
 constexpr size_t kLongest = 8192, kMostSums = size_t(256) << 20;
+
+// Rows of a key/value head up to which attn_rows_kernel serves a sequence, and sequences up to which a launch's own are looked up among them.
+constexpr size_t kFewRows = 64, kListed = 4096;
+
+// One kernel's share of a call and the join behind it.  nseq, rows: sequences and their rows of a key/value head, as far as the call tells
+// (what is split how follows from them; the kernels go by the device's arrays).
+int attend(smx_ctx* c, AttnArgs A, size_t nseq, size_t rows, size_t reach, bool few, bool bf16) {
+    int rc;
+    const int dc = A.kv.dim64 / 64;
+    const size_t all = A.kv.nseq, top = few ? std::min<size_t>((size_t)A.kv.max_rows * A.group, kFewRows) : (size_t)A.kv.max_rows * A.group;
+    A.tile_rows = few ? rows_per_tile(A.kv.dim64, rows) : 64 * tile_waves(c, A, nseq, rows, reach, bf16);
+    A.row_tiles = (int)((top + A.tile_rows - 1) / A.tile_rows);
+    // how many workgroups the sequences make without a split
+    const size_t groups = nseq * A.kv.kv_heads * ((rows + A.tile_rows - 1) / A.tile_rows);
+    // one to a CU, or two where that leaves each enough tokens; never a few more than that, which would wait for a round of their own
+    const size_t cus = c->num_cu, span = std::max<size_t>(reach, 1);
+    size_t split = std::max<size_t>(1, cus / groups);
+    if (span <= kWhole) split = 1;
+    else if (2 * cus / groups > split && span / (2 * cus / groups) >= (few ? kWorthFew : kWorthMany)) split = 2 * cus / groups;
+    // and no piece is longer than kLongest to 2 kLongest, as far as there is room for the pieces' sums
+    const size_t outputs = (size_t)A.kv.rows * A.q_heads, each = (size_t)A.kv.dim64 * 4 + 8;
+    split = std::max(split, std::min<size_t>(span * A.kv.dim64 / 128 / kLongest, kMostSums / (outputs * each)));
+    split = std::min<size_t>(split, kMaxPieces);
+    const size_t piece = std::max<size_t>(((span + split - 1) / split + 127) & ~size_t(127), 128);
+    A.piece = (int)std::min<size_t>(piece, size_t(1) << 30);
+    A.pieces = (int)std::max<size_t>((reach + piece - 1) / piece, 1);
+    if (A.pieces > 1) {
+        const size_t n = outputs * (size_t)A.pieces;
+        if ((rc = ensure(c, c->work, n * each)) != SMX_OK) return rc;
+        A.part = (float*)c->work.p;
+        A.part_ml = (float2*)(A.part + n * A.kv.dim64);
+    }
+    if (few) {
+        rc = launch_attn_rows(c, A, rows, bf16);
+    } else {
+        A.paired = groups * (size_t)A.pieces <= 2 * cus && A.pieces == 1;
+        const size_t z = A.listed ? std::min<size_t>(all, std::max<size_t>(1, (size_t)A.kv.rows * A.group / (A.above + 1))) : all;
+        const dim3 grid((unsigned)(A.kv.kv_heads * A.row_tiles), (unsigned)A.pieces, (unsigned)z);
+        ProfScope ps(c, "attn_tile");
+        switch (dc) {
+            case 1: rc = launch_dim<1>(c, A, grid, bf16); break;
+            case 2: rc = launch_dim<2>(c, A, grid, bf16); break;
+            case 3: rc = launch_dim<3>(c, A, grid, bf16); break;
+            default: rc = launch_dim<4>(c, A, grid, bf16); break;
+        }
+    }
+    if (rc != SMX_OK) return rc;
+    SMX_HIP(c, hipGetLastError());
+    if (A.pieces > 1 && !A.join) {
+        ProfScope ps(c, "attn_join");
+        if (A.pieces <= kJoinFew) {
+            const size_t units = 256 / (A.kv.dim64 / 4);
+            const dim3 jg((unsigned)((outputs + units - 1) / units));
+            if (bf16) hipLaunchKernelGGL(attn_join_few_kernel<true>, jg, dim3(256), 0, c->stream, A);
+            else hipLaunchKernelGGL(attn_join_few_kernel<false>, jg, dim3(256), 0, c->stream, A);
+        } else {
+            const dim3 jg((unsigned)A.kv.rows, (unsigned)A.q_heads);
+            if (bf16) hipLaunchKernelGGL(attn_join_kernel<true>, jg, dim3(256), 0, c->stream, A);
+            else hipLaunchKernelGGL(attn_join_kernel<false>, jg, dim3(256), 0, c->stream, A);
+        }
+        SMX_HIP(c, hipGetLastError());
+    }
+    return SMX_OK;
+}
+
+}  // namespace
+}  // namespace smx
+
+using namespace smx;
 
 extern "C" int smx_attn_dev(smx_ctx* c, const smx_kv_cache* cache, const smx_kv_batch* batch, int type, const void* q, size_t ldq, size_t q_heads,
                             float scale, size_t window, void* out, size_t ldo) {
@@ -417,61 +497,22 @@ extern "C" int smx_attn_dev(smx_ctx* c, const smx_kv_cache* cache, const smx_kv_
     A.scale = scale * kLog2e;
     const size_t per16 = bf16 ? 8 : 4;
     A.vec = cache->head_dim % 16 == 0 && ldq % per16 == 0 && ldo % per16 == 0 && (((uintptr_t)q | (uintptr_t)out) & 15) == 0;
-    const size_t tile_rows = batch->max_rows * (size_t)A.group;
-    const int dc = A.kv.dim64 / 64;
     // tokens in reach of one sequence's rows
     const size_t reach = window ? std::min<size_t>(A.kv.max_len, window + batch->max_rows + SMX_KV_BLOCK) : (size_t)A.kv.max_len;
-    const bool few = tile_rows <= 64;
-    A.tile_rows = few ? rows_per_tile(A.kv.dim64, tile_rows) : 64 * tile_waves(c, A, tile_rows, reach, bf16);
-    A.row_tiles = (int)((tile_rows + A.tile_rows - 1) / A.tile_rows);
-    // how many workgroups the sequences make without a split
-    const size_t groups = batch->nseq * cache->kv_heads * (size_t)A.row_tiles;
-    // one to a CU, or two where that leaves each enough tokens; never a few more than that, which would wait for a round of their own
-    const size_t cus = c->num_cu, span = std::max<size_t>(reach, 1);
-    size_t split = std::max<size_t>(1, cus / groups);
-    if (span <= kWhole) split = 1;
-    else if (2 * cus / groups > split && span / (2 * cus / groups) >= (few ? kWorthFew : kWorthMany)) split = 2 * cus / groups;
-    // and no piece is longer than kLongest to 2 kLongest, as far as there is room for the pieces' sums
-    const size_t sums = batch->rows * q_heads * ((size_t)A.kv.dim64 * 4 + 8);
-    split = std::max(split, std::min<size_t>(span * A.kv.dim64 / 128 / kLongest, kMostSums / sums));
-    split = std::min<size_t>(split, kMaxPieces);
-    const size_t piece = std::max<size_t>(((span + split - 1) / split + 127) & ~size_t(127), 128);
-    A.piece = (int)std::min<size_t>(piece, size_t(1) << 30);
-    A.pieces = (int)std::max<size_t>((reach + piece - 1) / piece, 1);
-    if (A.pieces > 1) {
-        const size_t n = batch->rows * q_heads * (size_t)A.pieces;
-        if ((rc = ensure(c, c->work, n * ((size_t)A.kv.dim64 * 4 + 8))) != SMX_OK) return rc;
-        A.part = (float*)c->work.p;
-        A.part_ml = (float2*)(A.part + n * A.kv.dim64);
+    const size_t most = batch->max_rows * (size_t)A.group;
+    A.upto = INT_MAX;
+    if (most <= kFewRows) return attend(c, A, batch->nseq, most, reach, true, bf16);
+    // Sequences of few rows in a call that has longer ones get the launch for few rows to themselves (in tiles of 64 or 128 rows, 63 decode
+    // steps beside a prompt chunk took 1169 us where each alone takes 100).  A call whose rows are all alike has none.
+    if (batch->rows < batch->nseq * batch->max_rows) {
+        AttnArgs F = A;
+        F.upto = (int)kFewRows;
+        if ((rc = attend(c, F, batch->nseq, A.group, reach, true, bf16)) != SMX_OK) return rc;
+        A.above = (int)kFewRows;
+        A.listed = batch->nseq <= kListed;
+        // the longer ones, were the others of one row and these of max_rows
+        const size_t longer = (batch->rows - std::min(batch->rows, batch->nseq) + batch->max_rows - 2) / (batch->max_rows - 1);
+        return attend(c, A, std::max<size_t>(longer, 1), most, reach, false, bf16);
     }
-    if (few) {
-        rc = launch_attn_rows(c, A, bf16);
-    } else {
-        A.paired = groups * (size_t)A.pieces <= 2 * (size_t)c->num_cu && A.pieces == 1;
-        const dim3 grid((unsigned)(cache->kv_heads * A.row_tiles), (unsigned)A.pieces, (unsigned)batch->nseq);
-        ProfScope ps(c, "attn_tile");
-        switch (dc) {
-            case 1: rc = launch_dim<1>(c, A, grid, bf16); break;
-            case 2: rc = launch_dim<2>(c, A, grid, bf16); break;
-            case 3: rc = launch_dim<3>(c, A, grid, bf16); break;
-            default: rc = launch_dim<4>(c, A, grid, bf16); break;
-        }
-    }
-    if (rc != SMX_OK) return rc;
-    SMX_HIP(c, hipGetLastError());
-    if (A.pieces > 1 && !A.join) {
-        ProfScope ps(c, "attn_join");
-        if (A.pieces <= kJoinFew) {
-            const size_t units = 256 / (A.kv.dim64 / 4);
-            const dim3 jg((unsigned)((batch->rows * q_heads + units - 1) / units));
-            if (bf16) hipLaunchKernelGGL(attn_join_few_kernel<true>, jg, dim3(256), 0, c->stream, A);
-            else hipLaunchKernelGGL(attn_join_few_kernel<false>, jg, dim3(256), 0, c->stream, A);
-        } else {
-            const dim3 jg((unsigned)batch->rows, (unsigned)q_heads);
-            if (bf16) hipLaunchKernelGGL(attn_join_kernel<true>, jg, dim3(256), 0, c->stream, A);
-            else hipLaunchKernelGGL(attn_join_kernel<false>, jg, dim3(256), 0, c->stream, A);
-        }
-        SMX_HIP(c, hipGetLastError());
-    }
-    return SMX_OK;
+    return attend(c, A, batch->nseq, most, reach, false, bf16);
 }

@@ -40,6 +40,8 @@ struct AttnArgs {
     unsigned* count;    // few rows: finished pieces of each (sequence, head, tile); 0 between launches
     int join;           // few rows: the last workgroup of a row tile to finish joins its pieces
     int tile_rows;
+    int above, upto;    // sequences of more than `above` and up to `upto` rows of a key/value head are this launch's
+    int listed;         // many rows: workgroups z serve the z-th of the sequences that are this launch's
     int q_heads, group, window;
     int piece;          // tokens per piece (a multiple of 32)
     int pieces;         // of the longest sequence
@@ -60,6 +62,8 @@ __device__ __forceinline__ Span seq_span(const AttnArgs& A, int s) {
     x.q = kv_seq(A.kv, s);
     x.first = A.window > 0 ? max(x.q.len - x.q.n - A.window + 1, 0) & ~(SMX_KV_BLOCK - 1) : 0;
     x.pieces = min((x.q.len - x.first + A.piece - 1) / A.piece, A.pieces);
+    const int64_t rows = (int64_t)x.q.n * A.group;
+    if (rows <= A.above || rows > A.upto) x.q.n = 0;
     return x;
 }
 
@@ -279,6 +283,6 @@ __device__ __forceinline__ void put_row(const AttnArgs& A, const RowAt& r, int p
 
 // Few rows of each sequence (attn_rows.hip): workgroups of the launch, and the launch with its join.
 int rows_per_tile(int dim64, size_t rows);
-int launch_attn_rows(smx_ctx* c, AttnArgs& A, bool bf16);
+int launch_attn_rows(smx_ctx* c, AttnArgs& A, size_t rows, bool bf16);   // rows: of a key/value head, as most sequences have them
 
 }  // namespace smx

@@ -41,7 +41,9 @@ __global__ __launch_bounds__(256, CT == 2 ? 2 : DC <= 1 ? 4 : DC == 2 ? 3 : 2) v
     extern __shared__ float wo[];   // [4][16][PITCH], one column tile at a time
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
     const int s = blockIdx.z, piece = blockIdx.y;
-    const int kvh = blockIdx.x % A.kv.kv_heads, tile = blockIdx.x / A.kv.kv_heads;
+    // (Sequences of fewer rows leave tiles empty: which of a sequence's workgroups those are goes round, since workgroups go to the parts of the
+    // chip in turn, and one in four at work would meet on a quarter of it: 188 us where all sequences of one row take 96.)
+    const int kvh = blockIdx.x % A.kv.kv_heads, tile = (blockIdx.x / A.kv.kv_heads + s) % A.row_tiles;
     const Span sp = seq_span(A, s);
     const int rows = sp.q.n * A.group;
     if (tile * ROWS >= rows) return;
@@ -292,10 +294,10 @@ int launch_dim(smx_ctx* c, const AttnArgs& A, dim3 grid, bool bf16) {
 
 int rows_per_tile(int dim64, size_t rows) { return rows <= 16 ? 16 : 16 * most_tiles(dim64 / 64); }
 
-int launch_attn_rows(smx_ctx* c, AttnArgs& A, bool bf16) {
+int launch_attn_rows(smx_ctx* c, AttnArgs& A, size_t rows, bool bf16) {
     int rc;
     const size_t items = (size_t)A.kv.nseq * A.kv.kv_heads * A.row_tiles;
-    A.join = A.pieces > 1 && A.pieces <= kJoinInside && (size_t)A.pieces * A.kv.max_rows * A.group <= (size_t)kJoinRows;
+    A.join = A.pieces > 1 && A.pieces <= kJoinInside && (size_t)A.pieces * rows <= (size_t)kJoinRows;
     if (A.join) {
         const size_t had = c->counts.cap;
         if ((rc = ensure(c, c->counts, items * 4)) != SMX_OK) return rc;

@@ -128,3 +128,33 @@ def test_one_long_sequence_among_many(accel, pkg, new, ty):
     got = got if ty == "f32" else R.from_bf16(got)
     # values of up to 128 * 0.02; the bounds that the tests of attention derive: 2e-5 of that, bf16 2^-8 of it
     assert np.abs(got - want).max() <= (2e-5 if ty == "f32" else 2.0 ** -8) * 128 * 0.02
+
+
+@pytest.mark.parametrize("nseq,chunks,ty,dim", [(3, [1], "f32", 64), (70, [5, 69], "f32", 64), (200, [0, 63, 64, 130, 199], "bf16", 128), (130, [], "f32", 80),
+                                                (4200, [17, 4199], "f32", 64)])
+def test_decode_steps_beside_prompt_chunks(accel, pkg, nseq, chunks, ty, dim):
+    """Sequences of one row (and of none) in a call with chunks of 33 rows and more: each kind has its own launch, the chunks wherever they
+    stand among the others."""
+    rng = np.random.default_rng(nseq)
+    kv, heads, page = 1, 2, 32
+    n = [1 if i % 11 else 0 for i in range(nseq)]
+    for j, c in enumerate(chunks):
+        n[c] = 33 + 7 * j
+    if not chunks:
+        n[40] = 32   # 64 rows of the key/value head: still few
+    lens = [m + int(x) for m, x in zip(n, rng.integers(0, 60, nseq))]
+    cache = R.Cache(sum(-(-m // page) for m in lens) + 1, page, kv, dim, seed=nseq)
+    cache.ks[:], cache.vs[:] = (rng.uniform(0.001, 0.02, cache.ks.shape).astype(np.float32) for _ in range(2))
+    table = R.tables(rng, cache.pages, page, lens)
+    q = rng.standard_normal((sum(n), heads, dim)).astype(np.float32)
+    raw = q if ty == "f32" else R.bf16(q)
+    q = q if ty == "f32" else R.from_bf16(raw)
+    want = R.attend(cache, table, lens, n, q, dim ** -0.5)
+    with R.Dev(accel) as dev:
+        d = R.OnDevice(pkg, dev, cache)
+        out = dev.put(np.full(raw.shape, 0x7fc0 if ty == "bf16" else np.nan, raw.dtype))
+        accel.attn_dev(d.handle, d.batch(table, lens, n, always_row0=True), dev.put(raw), heads, dim ** -0.5, out,
+                       dtype=pkg.DTYPE_F32 if ty == "f32" else pkg.DTYPE_BF16)
+        got = dev.get(out, raw.shape, raw.dtype)
+    got = got if ty == "f32" else R.from_bf16(got)
+    assert np.abs(got - want).max() <= (2e-5 if ty == "f32" else 2.0 ** -8) * 128 * 0.02
