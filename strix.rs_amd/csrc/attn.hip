@@ -504,7 +504,7 @@ extern "C" int smx_attn_dev(smx_ctx* c, const smx_kv_cache* cache, const smx_kv_
     if (most <= kFewRows) return attend(c, A, batch->nseq, most, reach, true, bf16);
     // Sequences of few rows in a call that has longer ones get the launch for few rows to themselves (in tiles of 64 or 128 rows, 63 decode
     // steps beside a prompt chunk took 1169 us where each alone takes 100).  A call whose rows are all alike has none.
-    if (batch->rows < batch->nseq * batch->max_rows) {
+    if (batch->rows < batch->nseq * batch->max_rows && (size_t)A.group <= kFewRows) {
         AttnArgs F = A;
         F.upto = (int)kFewRows;
         if ((rc = attend(c, F, batch->nseq, A.group, reach, true, bf16)) != SMX_OK) return rc;
