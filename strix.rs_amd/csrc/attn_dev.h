@@ -47,6 +47,7 @@ struct AttnArgs {
     int pieces;         // of the longest sequence
     int row_tiles;
     int paired;         // (see attn_tile_kernel)
+    int lone;           // few rows: workgroups of one wave
     float scale;        // times log2(e)
     int vec;            // rows may be read and written 16 bytes (bf16: 8) at a time
 };
@@ -181,7 +182,7 @@ struct Segment {
     float ks[kSegBlocks], vs[kSegBlocks];
     float top[4];   // largest value scale, per wave
 };
-static_assert(kSegBlocks == 256, "a block for each thread");
+static_assert(kSegBlocks == 256, "a block for each of 4 waves' threads");
 // (two steps, so that other loads can be on their way between the page table and the scales; a barrier follows)
 __device__ __forceinline__ int64_t find_segment(const AttnArgs& A, int s, int head, int blk0, int n) {
     return (int)threadIdx.x < n ? kv_block(A.kv, s, head, blk0 + threadIdx.x) : 0;
@@ -200,7 +201,8 @@ __device__ __forceinline__ void load_segment(const AttnArgs& A, Segment& seg, in
     for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
     if ((threadIdx.x & 63) == 0) seg.top[threadIdx.x >> 6] = top;
 }
-__device__ __forceinline__ float segment_top(const Segment& seg) { return fmaxf(fmaxf(seg.top[0], seg.top[1]), fmaxf(seg.top[2], seg.top[3])); }
+template <int WAVES>
+__device__ __forceinline__ float segment_top(const Segment& seg) { return WAVES == 1 ? seg.top[0] : fmaxf(fmaxf(seg.top[0], seg.top[1]), fmaxf(seg.top[2], seg.top[3])); }
 // Exponent that brings value scales up to `top` under 2^6 (times probabilities of up to 2^8 under 2^14).
 __device__ __forceinline__ int value_exponent(float top) {
     const int e = 5 - (int)((__float_as_uint(top) >> 23) & 255) + 127;

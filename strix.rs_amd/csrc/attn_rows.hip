@@ -30,15 +30,15 @@ __device__ __forceinline__ float row16_max(float v) {   // of 16 lanes
 }
 __device__ __forceinline__ float over(float L) { return L > 0.f ? 1.0f / L : L == L ? 0.f : L; }   // (a NaN stays one)
 
-// Workgroup (head and tile of 16 CT rows, piece of the context, sequence); its four waves take the piece's blocks in turn, straight
+// Workgroup (head and tile of 16 CT rows, piece of the context, sequence); its four waves (or one) take the piece's blocks in turn, straight
 // from memory into the matrix instructions' registers (one block ahead), and add up through LDS at the end.
-template <int DC, int CT, int NT, bool BF16>
-__global__ __launch_bounds__(256, CT == 2 ? 2 : DC <= 1 ? 4 : DC == 2 ? 3 : 2) void attn_rows_kernel(const AttnArgs A) {
-    constexpr int D64 = DC * 64, NO = DC * 4, ROWS = 16 * CT, PITCH = D64 + 4;
+template <int DC, int CT, int NT, int WAVES, bool BF16>
+__global__ __launch_bounds__(WAVES * 64, CT == 2 ? 2 : DC <= 1 ? 4 : DC == 2 ? 3 : 2) void attn_rows_kernel(const AttnArgs A) {
+    constexpr int D64 = DC * 64, NO = DC * 4, ROWS = 16 * CT, PITCH = D64 + 4, SEG = kSegBlocks * WAVES / 4;
     __shared__ Segment seg;
-    __shared__ float wm[4][ROWS], wl[4][ROWS];
+    __shared__ float wm[WAVES][ROWS], wl[WAVES][ROWS];
     __shared__ unsigned last;
-    extern __shared__ float wo[];   // [4][16][PITCH], one column tile at a time
+    extern __shared__ float wo[];   // [WAVES][16][PITCH], one column tile at a time
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
     const int s = blockIdx.z, piece = blockIdx.y;
     // (Sequences of fewer rows leave tiles empty: which of a sequence's workgroups those are goes round, since workgroups go to the parts of the
@@ -49,7 +49,7 @@ __global__ __launch_bounds__(256, CT == 2 ? 2 : DC <= 1 ? 4 : DC == 2 ? 3 : 2) v
     if (tile * ROWS >= rows) return;
     if (piece >= sp.pieces) {
         if (piece == 0) {   // a sequence without a token in the cache
-            for (int it = threadIdx.x; it < min(ROWS, rows - tile * ROWS) * (D64 / 4); it += 256) {
+            for (int it = threadIdx.x; it < min(ROWS, rows - tile * ROWS) * (D64 / 4); it += WAVES * 64) {
                 const int r = it / (D64 / 4);
                 store_out<BF16>(A, row_at(A, sp.q, kvh, tile * ROWS + r), (it - r * (D64 / 4)) * 4, v4f{0.f, 0.f, 0.f, 0.f});
             }
@@ -85,8 +85,8 @@ __global__ __launch_bounds__(256, CT == 2 ? 2 : DC <= 1 ? 4 : DC == 2 ? 3 : 2) v
 #pragma unroll
         for (int i = 0; i < NO; i++) o[ct][i] = v4f{0.f, 0.f, 0.f, 0.f};
     }
-    for (int c0 = b0; c0 < b1; c0 += kSegBlocks) {
-        const int n = min(kSegBlocks, b1 - c0);
+    for (int c0 = b0; c0 < b1; c0 += SEG) {
+        const int n = min(SEG, b1 - c0);
         if (c0 != b0) __syncthreads();
         load_segment(A, seg, find_segment(A, s, kvh, c0, n), n);
         __syncthreads();
@@ -94,7 +94,7 @@ __global__ __launch_bounds__(256, CT == 2 ? 2 : DC <= 1 ? 4 : DC == 2 ? 3 : 2) v
             fetch(kb, A.kv.k, wave);
             fetch(vb, A.kv.v, wave);
         }
-        const int e = value_exponent(segment_top(seg));
+        const int e = value_exponent(segment_top<WAVES>(seg));
         if (e != vexp) {
             const float f = pow2(min(max(e - vexp, -126), 127));
             for (int ct = 0; ct < CT; ct++)
@@ -103,7 +103,7 @@ __global__ __launch_bounds__(256, CT == 2 ? 2 : DC <= 1 ? 4 : DC == 2 ? 3 : 2) v
             vexp = e;
         }
         const float vup = pow2(vexp);
-        for (int i = wave; i < n; i += 4) {
+        for (int i = wave; i < n; i += WAVES) {
             v4f sc[CT][2];
 #pragma unroll
             for (int tt = 0; tt < 2; tt++) {
@@ -124,7 +124,7 @@ __global__ __launch_bounds__(256, CT == 2 ? 2 : DC <= 1 ? 4 : DC == 2 ? 3 : 2) v
                 }
             }
             const float ks = seg.ks[i], vs = seg.vs[i] * vup;
-            const int next = i + 4;
+            const int next = i + WAVES;
             if (next < n) fetch(kb, A.kv.k, next);
             const int tok = (c0 + i) * SMX_KV_BLOCK;
             const bool edge = tok + SMX_KV_BLOCK - 1 > all_hi || tok < all_lo;
@@ -186,13 +186,15 @@ __global__ __launch_bounds__(256, CT == 2 ? 2 : DC <= 1 ? 4 : DC == 2 ? 3 : 2) v
     for (int ct = 0; ct < CT; ct++) {
         __syncthreads();
         const int r = ct * 16 + (lane & 15);
-        const float M = fmaxf(fmaxf(wm[0][r], wm[1][r]), fmaxf(wm[2][r], wm[3][r]));
+        float M = wm[0][r];
+#pragma unroll
+        for (int v = 1; v < WAVES; v++) M = fmaxf(M, wm[v][r]);
         const float f = __builtin_amdgcn_exp2f(m[ct] - M) * down;
 #pragma unroll
         for (int i = 0; i < NO; i++) *(v4f*)&wo[(wave * 16 + (lane & 15)) * PITCH + i * 16 + g * 4] = o[ct][i] * f;
         float L = 0.f;
 #pragma unroll
-        for (int v = 0; v < 4; v++) L += wl[v][r] * __builtin_amdgcn_exp2f(wm[v][r] - M);
+        for (int v = 0; v < WAVES; v++) L += wl[v][r] * __builtin_amdgcn_exp2f(wm[v][r] - M);
         __syncthreads();
         if (!at[ct].live) continue;
         const int64_t mine = ((int64_t)at[ct].row * A.q_heads + at[ct].head) * A.pieces + piece;
@@ -200,13 +202,13 @@ __global__ __launch_bounds__(256, CT == 2 ? 2 : DC <= 1 ? 4 : DC == 2 ? 3 : 2) v
             give(&A.part_ml[mine].x, M);
             give(&A.part_ml[mine].y, L);
         }
-        // wave w writes channels [w * D64 / 4, ...)
+        // wave w writes channels [w * D64 / WAVES, ...)
 #pragma unroll
-        for (int i = 0; i < DC; i++) {
-            const int d = (wave * DC + i) * 16 + g * 4;
+        for (int i = 0; i < NO / WAVES; i++) {
+            const int d = (wave * (NO / WAVES) + i) * 16 + g * 4;
             v4f acc = *(v4f*)&wo[(lane & 15) * PITCH + d];
 #pragma unroll
-            for (int v = 1; v < 4; v++) acc += *(v4f*)&wo[(v * 16 + (lane & 15)) * PITCH + d];
+            for (int v = 1; v < WAVES; v++) acc += *(v4f*)&wo[(v * 16 + (lane & 15)) * PITCH + d];
             if (sp.pieces == 1) {
                 store_out<BF16>(A, at[ct], d, acc * over(L));
             } else {
@@ -231,7 +233,7 @@ __global__ __launch_bounds__(256, CT == 2 ? 2 : DC <= 1 ? 4 : DC == 2 ? 3 : 2) v
     // factors of all (row, piece) first, so that nothing stands between the loads of the sums
     const int live = min(ROWS, rows - tile * ROWS);
     float2* factor = (float2*)wo;   // [ROWS][kJoinInside], x: the factor, y: the piece's share of the row's sum
-    for (int it = threadIdx.x; it < live * kJoinInside; it += 256) {
+    for (int it = threadIdx.x; it < live * kJoinInside; it += WAVES * 64) {
         const int r = it / kJoinInside, i = it - r * kJoinInside;
         float2 ml = make_float2(kNoMax, 0.f);
         if (i < sp.pieces) {
@@ -244,7 +246,7 @@ __global__ __launch_bounds__(256, CT == 2 ? 2 : DC <= 1 ? 4 : DC == 2 ? 3 : 2) v
         factor[it] = make_float2(f, ml.y * f);
     }
     __syncthreads();
-    constexpr int QUADS = D64 / 4, GROUPS = 256 / QUADS;
+    constexpr int QUADS = D64 / 4, GROUPS = WAVES * 64 / QUADS;
     const int gr = threadIdx.x / QUADS, d = (threadIdx.x - gr * QUADS) * 4;
     for (int r = gr; r < live && gr < GROUPS; r += GROUPS) {
         const RowAt x = row_at(A, sp.q, kvh, tile * ROWS + r);
@@ -274,20 +276,24 @@ __global__ __launch_bounds__(256) void clear_kernel(unsigned* p, size_t n) {
     if (i < n) p[i] = 0;
 }
 
-template <int DC, int CT, int NT, bool BF16>
+template <int DC, int CT, int NT, int WAVES, bool BF16>
 int launch(smx_ctx* c, const AttnArgs& A, dim3 grid) {
-    const size_t lds = 4 * 16 * (DC * 64 + 4) * 4;
+    const size_t lds = WAVES * 16 * (DC * 64 + 4) * 4;
     int rc;
-    if ((rc = set_dyn_lds(c, attn_rows_kernel<DC, CT, NT, BF16>, lds)) != SMX_OK) return rc;
-    hipLaunchKernelGGL((attn_rows_kernel<DC, CT, NT, BF16>), grid, dim3(256), lds, c->stream, A);
+    if ((rc = set_dyn_lds(c, attn_rows_kernel<DC, CT, NT, WAVES, BF16>, lds)) != SMX_OK) return rc;
+    hipLaunchKernelGGL((attn_rows_kernel<DC, CT, NT, WAVES, BF16>), grid, dim3(WAVES * 64), lds, c->stream, A);
     return SMX_OK;
 }
 // Two column tiles to a wave where their registers leave two waves a SIMD (and the second tile's products share the widened bytes).
 constexpr int most_tiles(int dc) { return dc <= 2 ? 2 : 1; }
+template <int DC, int WAVES>
+int launch_tiles(smx_ctx* c, const AttnArgs& A, dim3 grid, bool bf16) {
+    if (A.tile_rows == 16) return bf16 ? launch<DC, 1, 1, WAVES, true>(c, A, grid) : launch<DC, 1, 2, WAVES, false>(c, A, grid);
+    return bf16 ? launch<DC, most_tiles(DC), 1, WAVES, true>(c, A, grid) : launch<DC, most_tiles(DC), 2, WAVES, false>(c, A, grid);
+}
 template <int DC>
 int launch_dim(smx_ctx* c, const AttnArgs& A, dim3 grid, bool bf16) {
-    if (A.tile_rows == 16) return bf16 ? launch<DC, 1, 1, true>(c, A, grid) : launch<DC, 1, 2, false>(c, A, grid);
-    return bf16 ? launch<DC, most_tiles(DC), 1, true>(c, A, grid) : launch<DC, most_tiles(DC), 2, false>(c, A, grid);
+    return A.lone ? launch_tiles<DC, 1>(c, A, grid, bf16) : launch_tiles<DC, 4>(c, A, grid, bf16);
 }
 
 }  // namespace

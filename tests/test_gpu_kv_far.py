@@ -158,3 +158,28 @@ def test_decode_steps_beside_prompt_chunks(accel, pkg, nseq, chunks, ty, dim):
         got = dev.get(out, raw.shape, raw.dtype)
     got = got if ty == "f32" else R.from_bf16(got)
     assert np.abs(got - want).max() <= (2e-5 if ty == "f32" else 2.0 ** -8) * 128 * 0.02
+
+
+@pytest.mark.parametrize("ty,dim,new,window", [("f32", 64, 1, 0), ("bf16", 128, 1, 50), ("f32", 192, 2, 0), ("bf16", 256, 3, 0), ("f32", 80, 4, 33)])
+def test_many_short_sequences(accel, pkg, ty, dim, new, window):
+    """Enough of them for a wave each: lengths from none to several hundred."""
+    rng = np.random.default_rng(dim + new)
+    kv, heads, page, nseq = 8, 32, 32, 140
+    lens = [int(x) for x in rng.integers(0, 60, nseq)]
+    lens[3], lens[70], lens[139] = 0, 470, 256
+    n = [new if new > 1 else 1] * nseq
+    cache = R.Cache(sum(-(-m // page) for m in lens) + 1, page, kv, dim, seed=dim)
+    cache.ks[:], cache.vs[:] = (rng.uniform(0.001, 0.02, cache.ks.shape).astype(np.float32) for _ in range(2))
+    table = R.tables(rng, cache.pages, page, lens)
+    q = rng.standard_normal((sum(n), heads, dim)).astype(np.float32)
+    raw = q if ty == "f32" else R.bf16(q)
+    q = q if ty == "f32" else R.from_bf16(raw)
+    want = R.attend(cache, table, lens, n, q, dim ** -0.5, window)
+    with R.Dev(accel) as dev:
+        d = R.OnDevice(pkg, dev, cache)
+        out = dev.put(np.full(raw.shape, 0x7fc0 if ty == "bf16" else np.nan, raw.dtype))
+        accel.attn_dev(d.handle, d.batch(table, lens, n), dev.put(raw), heads, dim ** -0.5, out, window=window,
+                       dtype=pkg.DTYPE_F32 if ty == "f32" else pkg.DTYPE_BF16)
+        got = dev.get(out, raw.shape, raw.dtype)
+    got = got if ty == "f32" else R.from_bf16(got)
+    assert np.abs(got - want).max() <= (2e-5 if ty == "f32" else 2.0 ** -8) * 128 * 0.02
