@@ -402,10 +402,13 @@ constexpr size_t kWorthFew = 512, kWorthMany = 256;
 // tokens 8.8 / 10.2, of 350 9.8 / 10.3, of 600 11.8 / 11.4; 64 rows of 200 15.6 / 22.3, of 350 19.7 / 22.7, of 600 26.4 / 26.1.
 constexpr size_t kWhole = 384;
 
-// Contexts up to which many (sequence, key/value head) pairs, four for each CU, take a wave each: four waves of a pair have a block or two each
-// and then their sums to put together.  Four waves / one, one row of 32/8 heads of 128 channels: 128 sequences of 50 tokens 15 / 10, of
-// 200 21 / 16, 1000 of 100 98 / 53, of 300 154 / 133, of 500 208 / 203, of 800 307 / 305, of 20..800 188 / 192; 96 of 200 16 / 16.
-constexpr size_t kLone = 512;
+// Contexts up to which (sequence, key/value head) pairs, where they are more than workgroups of four waves have places at once, take a wave
+// each: four waves of a pair have a block or two each and then their sums to put together.  Four waves / one, one row of 32/8 heads of
+// 128 channels: 128 sequences of 50 tokens 15 / 10, of 200 21 / 16, 1000 of 100 98 / 53, of 300 154 / 133, of 500 208 / 203, of 800
+// 307 / 305, of 20..800 188 / 192.  A window makes longer contexts alike too; there single waves win where four would begin a second round
+// that does not fill the chip (16/8 heads of 256 bf16 channels, window of 1024, 80 / 96 / 100 / 128 / 150 sequences: 75 / 67, 83 / 75,
+// 87 / 81, 99 / 98, 117 / 121).
+constexpr size_t kLone = 512, kLoneWindow = 1152;
 // Tokens of 128 channels of a piece, however many sequences there are: the call knows the longest only, and one long sequence among short ones
 // would keep a few workgroups busy for long after the others.  One row each of 64 sequences of 500 tokens and one of 131072: 145 us, without
 // 1163; 64 of 33..32768 430 / 462; where all are alike it costs a little: 64 of 16384 394 / 370.
@@ -433,7 +436,8 @@ int attend(smx_ctx* c, AttnArgs A, size_t nseq, size_t rows, size_t reach, bool 
     const size_t outputs = (size_t)A.kv.rows * A.q_heads, each = (size_t)A.kv.dim64 * 4 + 8;
     split = std::max(split, std::min<size_t>(span * A.kv.dim64 / 128 / kLongest, kMostSums / (outputs * each)));
     split = std::min<size_t>(split, kMaxPieces);
-    A.lone = few && groups >= 4 * cus && span <= kLone;
+    const size_t places = cus * rows_residents(A.kv.dim64, A.tile_rows);
+    A.lone = few && groups > places && (span <= kLone || (A.window > 0 && 4 * groups >= 5 * places && groups <= 2 * places && span <= kLoneWindow));
     const size_t piece = std::max<size_t>(((span + split - 1) / split + 127) & ~size_t(127), 128);
     A.piece = (int)std::min<size_t>(piece, size_t(1) << 30);
     A.pieces = (int)std::max<size_t>((reach + piece - 1) / piece, 1);

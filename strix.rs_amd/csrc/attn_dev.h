@@ -285,6 +285,7 @@ __device__ __forceinline__ void put_row(const AttnArgs& A, const RowAt& r, int p
 
 // Few rows of each sequence (attn_rows.hip): workgroups of the launch, and the launch with its join.
 int rows_per_tile(int dim64, size_t rows);
+int rows_residents(int dim64, int tile_rows);   // workgroups of four waves on a CU
 int launch_attn_rows(smx_ctx* c, AttnArgs& A, size_t rows, bool bf16);   // rows: of a key/value head, as most sequences have them
 
 }  // namespace smx

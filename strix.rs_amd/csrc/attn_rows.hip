@@ -30,10 +30,13 @@ __device__ __forceinline__ float row16_max(float v) {   // of 16 lanes
 }
 __device__ __forceinline__ float over(float L) { return L > 0.f ? 1.0f / L : L == L ? 0.f : L; }   // (a NaN stays one)
 
+// Waves on a SIMD: what the registers leave.
+constexpr int residents(int dc, int ct) { return ct == 2 ? 2 : dc <= 1 ? 4 : dc == 2 ? 3 : 2; }
+
 // Workgroup (head and tile of 16 CT rows, piece of the context, sequence); its four waves (or one) take the piece's blocks in turn, straight
 // from memory into the matrix instructions' registers (one block ahead), and add up through LDS at the end.
 template <int DC, int CT, int NT, int WAVES, bool BF16>
-__global__ __launch_bounds__(WAVES * 64, CT == 2 ? 2 : DC <= 1 ? 4 : DC == 2 ? 3 : 2) void attn_rows_kernel(const AttnArgs A) {
+__global__ __launch_bounds__(WAVES * 64, residents(DC, CT)) void attn_rows_kernel(const AttnArgs A) {
     constexpr int D64 = DC * 64, NO = DC * 4, ROWS = 16 * CT, PITCH = D64 + 4, SEG = kSegBlocks * WAVES / 4;
     __shared__ Segment seg;
     __shared__ float wm[WAVES][ROWS], wl[WAVES][ROWS];
@@ -299,6 +302,8 @@ int launch_dim(smx_ctx* c, const AttnArgs& A, dim3 grid, bool bf16) {
 }  // namespace
 
 int rows_per_tile(int dim64, size_t rows) { return rows <= 16 ? 16 : 16 * most_tiles(dim64 / 64); }
+
+int rows_residents(int dim64, int tile_rows) { return residents(dim64 / 64, tile_rows / 16); }
 
 int launch_attn_rows(smx_ctx* c, AttnArgs& A, size_t rows, bool bf16) {
     int rc;
