@@ -622,7 +622,9 @@ __device__ Last cut_by_steps(const SampleArgs& A, const Ask& q, const Row& r, Re
             found[0] = first + e - 1;
         }
         __syncthreads();
-        return (unsigned)found[0];
+        const unsigned at = (unsigned)found[0];
+        __syncthreads();   // (the next cut writes found again)
+        return at;
     };
     // the last of the bound's tokens, in order, with less than the limit in front of it: `limit` tokens, or (weighed) top_p of their weight
     auto cut = [&](Last bound, bool weighed, unsigned long long limit) {
