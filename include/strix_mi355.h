@@ -286,7 +286,7 @@ typedef struct smx_kv_batch {
     const int32_t* table;  /* device [nseq][table_ld]: the page of each page_tokens tokens */
     size_t table_ld;
     size_t rows;           /* rows of all sequences (nseq when row0 is NULL) */
-    size_t max_rows;       /* at least every n_s (1 when row0 is NULL) */
+    size_t max_rows;       /* at least every n_s (1 when row0 is NULL); 0 only where rows is */
     size_t max_len;        /* at least every len */
 } smx_kv_batch;
 /* Position rotation of the first rot_dim (even) channels: (a, b) -> (a cos - b sin, a sin + b cos) with (a, b) channels

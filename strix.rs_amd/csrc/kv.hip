@@ -20,7 +20,7 @@ int kv_args(smx_ctx* c, const char* who, const smx_kv_cache* cache, const smx_kv
     if (b->table_ld == 0) return fail(c, SMX_ERR_ARG, "%s: empty page table", who);
     if (!b->row0 && (b->rows != b->nseq || b->max_rows != 1))
         return fail(c, SMX_ERR_ARG, "%s: %zu rows (at most %zu each) of %zu sequences without row0", who, b->rows, b->max_rows, b->nseq);
-    if (b->max_rows > b->rows) return fail(c, SMX_ERR_ARG, "%s: max_rows %zu of %zu rows", who, b->max_rows, b->rows);
+    if (b->max_rows > b->rows || (b->max_rows == 0 && b->rows > 0)) return fail(c, SMX_ERR_ARG, "%s: max_rows %zu of %zu rows", who, b->max_rows, b->rows);
     if (b->nseq > 65535 || b->rows > (size_t(1) << 24) || b->max_len > (size_t(1) << 28) || b->table_ld > (size_t(1) << 26) || cache->pages > INT_MAX)
         return fail(c, SMX_ERR_LIMIT, "%s: %zu sequences (65535), %zu rows (2^24), %zu tokens (2^28), %zu pages (2^31 - 1)", who, b->nseq, b->rows,
                     b->max_len, cache->pages);

@@ -1,0 +1,35 @@
+"""The host side of the cache and attention calls on the test double of the HIP runtime: what they refuse, and the memory they ask for."""
+import pytest
+
+from test_host_runtime import fake, run  # noqa: F401 (fixtures)
+
+SETUP = """
+a = pkg.Mi355WeightAccel(0)
+room = a.dev_alloc(1 << 20)
+KV, HEADS, DIM = 2, 8, 64
+cache = pkg.KvCache(64, 64, KV, DIM, room, room, room, room)
+def batch(nseq, rows, max_rows, max_len=4000):
+    return pkg.KvBatch(nseq, room, room, 64, max_len, row0=room, rows=rows, max_rows=max_rows)
+def refused(f, code=-1):
+    try:
+        f()
+    except pkg.SmxError as e:
+        assert e.code == code, e
+    else:
+        raise AssertionError("not refused")
+"""
+
+
+def test_no_rows_to_a_sequence(run):   # noqa: F811
+    """Rows of which no sequence may have one."""
+    run(SETUP + """
+for rows in (1, 3, 500):
+    b = batch(3, rows, 0)
+    refused(lambda: a.attn_dev(cache, b, room, HEADS, 1.0, room))
+    refused(lambda: a.kv_append_dev(cache, b, room, room))
+    refused(lambda: a.kv_read_dev(cache, b, room, room))
+b = batch(3, 0, 0)                                   # a step without a row is a step
+a.attn_dev(cache, b, room, HEADS, 1.0, room)
+a.kv_append_dev(cache, b, room, room)
+a.kv_read_dev(cache, b, room, room)
+""")
