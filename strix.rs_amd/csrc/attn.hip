@@ -507,7 +507,7 @@ extern "C" int smx_attn_dev(smx_ctx* c, const smx_kv_cache* cache, const smx_kv_
     const size_t per16 = bf16 ? 8 : 4;
     A.vec = cache->head_dim % 16 == 0 && ldq % per16 == 0 && ldo % per16 == 0 && (((uintptr_t)q | (uintptr_t)out) & 15) == 0;
     // tokens in reach of one sequence's rows
-    const size_t reach = window ? std::min<size_t>(A.kv.max_len, window + batch->max_rows + SMX_KV_BLOCK) : (size_t)A.kv.max_len;
+    const size_t reach = window ? std::min<size_t>(A.kv.max_len, (size_t)A.window + batch->max_rows + SMX_KV_BLOCK) : (size_t)A.kv.max_len;
     const size_t most = batch->max_rows * (size_t)A.group;
     A.upto = INT_MAX;
     if (most <= kFewRows) return attend(c, A, batch->nseq, most, reach, true, bf16);
