@@ -315,7 +315,8 @@ int smx_kv_append_dev(smx_ctx* ctx, const smx_kv_cache* cache, const smx_kv_batc
 int smx_kv_read_dev(smx_ctx* ctx, const smx_kv_cache* cache, const smx_kv_batch* batch, float* k_dev, float* v_dev);
 /* out = softmax(scale * q K^T) V for each query row and head over the row's own sequence: keys at positions up to the row's own
  * and, with window > 0, only the last `window` of them.  q, out: [rows][q_heads][head_dim] of `type`, ldq, ldo elements from row
- * to row; q_heads a multiple of kv_heads, query heads of one group next to each other.  A row that sees no key gives zeros.
+ * to row; q_heads a multiple of kv_heads, query heads of one group next to each other; scale of either sign.  A row that sees no
+ * key gives zeros.
  * fp32 rows are computed to fp32 accuracy (queries and probabilities as two f16 terms each on the matrix cores), bf16 rows with one
  * f16 term; statistics and sums are fp32.  A row's result depends on its own sequence and on the sizes of the call (nseq, rows,
  * max_rows, max_len, which set how a long sequence is split), not on the other sequences.  Capturable. */

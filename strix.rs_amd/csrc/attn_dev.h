@@ -112,7 +112,8 @@ __device__ __forceinline__ float row_sum(float v) {
 }
 
 // The query rows of one column tile as the B operand of S^T = K Q^T: lane (row lane % 16, g) holds channels 64 c + 16 g + 0..15 of
-// its row, scaled by a power of two; *unit is what a product of them with codes times a key scale is multiplied by.
+// its row, times a power of two and the sign of the call's scale; *unit (not negative) is what a product of them with codes times
+// a key scale is multiplied by.
 // (load_query: the channels as they are; set_query: the operand.)
 template <int DC, bool BF16>
 __device__ __forceinline__ void load_query(const AttnArgs& A, bool live, int64_t at, float (&x)[DC][16]) {
@@ -158,8 +159,9 @@ __device__ __forceinline__ void set_query(const AttnArgs& A, const float (&x)[DC
     // 2^e with top * 2^e in [2^14, 2^15): f16's largest power of two; 0, inf and subnormal maxima keep e in range
     int e = 14 - (int)((__float_as_uint(top) >> 23) & 255) + 127;
     e = min(max(e, -115), 120);
-    const float up = __uint_as_float((unsigned)(e + 127) << 23);
-    *unit = A.scale * __uint_as_float((unsigned)(127 - e) << 23);
+    // (the sign of the call's scale goes into the operand, so that a larger product is a larger score)
+    const float up = copysignf(__uint_as_float((unsigned)(e + 127) << 23), A.scale);
+    *unit = fabsf(A.scale) * __uint_as_float((unsigned)(127 - e) << 23);
 #pragma unroll
     for (int c = 0; c < DC; c++)
 #pragma unroll

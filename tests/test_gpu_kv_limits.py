@@ -48,3 +48,18 @@ def test_window_without_an_end(accel, pkg, new):
         got = _attention(accel, pkg, cache, table, [length], [new], raw, "f32", dim ** -0.5, window=window)
         # (another split is another order of the same sums)
         assert np.abs(got - none).max() <= 2 * TOL["f32"] * 128 * 0.02, window
+
+
+@pytest.mark.parametrize("ty,dim,new", [("f32", 64, 1), ("f32", 128, 150), ("bf16", 128, 150), ("f32", 256, 70), ("bf16", 80, 3)])
+@pytest.mark.parametrize("scale", [-0.125, -1.0, 0.0])
+def test_scale_of_either_sign(accel, pkg, ty, dim, new, scale):
+    """Scores of up to hundreds, so that a maximum taken for a minimum leaves every range."""
+    rng = np.random.default_rng(dim + new)
+    kv, heads, length = 1, 4, 700
+    cache = _random_cache(rng, 64, kv, dim, length)
+    table = R.tables(rng, cache.pages, 64, [length])
+    q, raw = _queries(rng, ty, new, heads, dim)
+    got = _attention(accel, pkg, cache, table, [length], [new], raw, ty, scale)
+    want = R.attend(cache, table, [length], [new], q, scale)
+    # |scores| up to 0.02 * 128 * 3 * sqrt(dim) * |scale|: eight times the tests' 31 at the largest, and so is their rounding
+    assert np.abs(got - want).max() <= (8 * TOL[ty] if ty == "f32" else TOL[ty]) * 128 * 0.02
