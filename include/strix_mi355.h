@@ -317,9 +317,10 @@ int smx_kv_read_dev(smx_ctx* ctx, const smx_kv_cache* cache, const smx_kv_batch*
  * and, with window > 0, only the last `window` of them.  q, out: [rows][q_heads][head_dim] of `type`, ldq, ldo elements from row
  * to row; q_heads a multiple of kv_heads, query heads of one group next to each other; scale of either sign.  A row that sees no
  * key gives zeros.
- * fp32 rows are computed to fp32 accuracy (queries and probabilities as two f16 terms each on the matrix cores), bf16 rows with one
- * f16 term; statistics and sums are fp32.  A row's result depends on its own sequence and on the sizes of the call (nseq, rows,
- * max_rows, max_len, which set how a long sequence is split), not on the other sequences.  Capturable. */
+ * fp32 rows are computed to fp32 accuracy (queries and probabilities as two f16 terms each on the matrix cores; errors are relative
+ * to the row's largest probability times value, as long as the value scales of a sequence are above 2^-90 and within 2^100 of each
+ * other), bf16 rows with one f16 term; statistics and sums are fp32.  A row's result depends on its own sequence and on the sizes of
+ * the call (nseq, rows, max_rows, max_len, which set how a long sequence is split), not on the other sequences.  Capturable. */
 int smx_attn_dev(smx_ctx* ctx, const smx_kv_cache* cache, const smx_kv_batch* batch, int type, const void* q_dev, size_t ldq,
                  size_t q_heads, float scale, size_t window, void* out_dev, size_t ldo);
 

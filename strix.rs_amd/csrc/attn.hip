@@ -34,7 +34,8 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(const AttnArgs A) {
     constexpr int UNITS = TB * 2 * DC, PER = (UNITS + 3) / 4;      // 1 KB units of a tile's keys (and values); of them a wave's
     constexpr int KEYS = TB * 2 * KF * 64, TILE = KEYS + TB * NO * 64;   // 16-byte words: keys [block][token / 16][KF][lane], values [block][NO][lane]
     __shared__ Segment seg;
-    extern __shared__ uint4 stage[];   // [2][TILE]
+    __shared__ float4 value[kSegBlocks];   // of a block's value scale: exponent e, log2(scale 2^(kLift - e)), 1 / (scale 2^kLift), the scale itself
+    extern __shared__ uint4 stage[];       // [2][TILE]
     const int s = A.listed ? nth_sequence(A, blockIdx.z) : blockIdx.z, piece = blockIdx.y;
     if (s < 0) return;
     const int kvh = blockIdx.x % A.kv.kv_heads;
@@ -74,22 +75,21 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(const AttnArgs A) {
     const int wfirst = pos0 + wrow0 / A.group, wlast = pos0 + min(wrow0 + 16 * CT - 1, rows - 1) / A.group;
     const int all_hi = wfirst, all_lo = A.window > 0 ? wlast - A.window + 1 : 0;
     const int any_hi = wrow0 < rows ? wlast : -1, any_lo = A.window > 0 ? wfirst - A.window + 1 : 0;
-    int vexp = 0;
+    float least = 0.f;
     const int b0 = tok0 / SMX_KV_BLOCK, b1 = tok1 > tok0 ? (tok1 + SMX_KV_BLOCK - 1) / SMX_KV_BLOCK : b0;
     for (int c0 = b0; c0 < b1; c0 += kSegBlocks) {
         const int n = min(kSegBlocks, b1 - c0), tiles = (n + TB - 1) / TB;
         __syncthreads();
         load_segment(A, seg, find_segment(A, s, kvh, c0, n), n);
         __syncthreads();
-        const int e = value_exponent(segment_top<4>(seg));
-        if (e != vexp) {
-            const float f = pow2(min(max(e - vexp, -126), 127));
-            for (int ct = 0; ct < CT; ct++)
-#pragma unroll
-                for (int i = 0; i < NO; i++) o[ct][i] *= f;
-            vexp = e;
+        least = fmaxf(least, least_scale(segment_top<4>(seg)));
+        if ((int)threadIdx.x < n) {
+            // (a value scale of 0 stands for codes of 0; a NaN one is for the rows that see a token of the block)
+            const float scale = seg.vs[threadIdx.x], vs = fmaxf(scale, least);
+            const int e = exponent_of(vs);
+            value[threadIdx.x] = make_float4((float)e, __builtin_amdgcn_logf(vs * pow2(kLift - e)), __builtin_amdgcn_rcpf(vs) * (1.0f / (1 << kLift)), scale);
         }
-        const float vup = pow2(vexp);
+        __syncthreads();
         uint4 kb[PER], vb[PER];
         // this wave's units of a tile: u = wave + 4 j (a last tile's missing block is its first again, and masked)
         auto fetch = [&](int t) {
@@ -137,8 +137,8 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(const AttnArgs A) {
                         for (int ct = 0; ct < CT; ct++) sc[ct][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[k], qf[ct][nt][k], sc[ct][tt], 0, 0, 0);
             }
         };
-        // probabilities times value scale of block i, 2^(scores * f + base), and their product with its values; the sums of
-        // probabilities take the scale out again (per_vs)
+        // weights of block i, 2^(scores * f + base), and their product with its values; the sums of probabilities take the value scale
+        // out again (per_vs)
         auto weigh = [&](const v4f (&sc)[CT][2], const float (&f)[CT], const float (&base)[CT], float per_vs, float poison, int i) {
             v8h pf[CT][NT];
 #pragma unroll
@@ -232,9 +232,8 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(const AttnArgs A) {
             const int tok = (c0 + i) * SMX_KV_BLOCK;
             const bool edge = tok + SMX_KV_BLOCK - 1 > all_hi || tok < all_lo;
             const float ks = seg.ks[i];
-            // a value scale of 0 stands for codes of 0; a NaN one is for the rows that see a token of the block
-            const float scale = seg.vs[i] * vup, vs = fmaxf(scale, 0x1p-60f), poison = scale == scale ? 0.f : scale;
-            const float log_vs = __builtin_amdgcn_logf(vs), per_vs = __builtin_amdgcn_rcpf(vs);
+            const float4 vs = value[i];
+            const float exponent = vs.x, log_rest = vs.y, per_vs = vs.z, poison = vs.w == vs.w ? 0.f : vs.w;
             float f[CT], base[CT], mx[CT];
 #pragma unroll
             for (int ct = 0; ct < CT; ct++) {
@@ -251,11 +250,11 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(const AttnArgs A) {
                 mx[ct] = kNoMax;
 #pragma unroll
                 for (int j = 0; j < 8; j++) mx[ct] = fmaxf(mx[ct], cur[ct][j >> 2][j & 3]);
-                mx[ct] = row_max(mx[ct]) * f[ct];
+                mx[ct] = row_max(mx[ct]) * f[ct] + exponent;
             }
             rescale<CT, NO>(mx, m, l, o);
 #pragma unroll
-            for (int ct = 0; ct < CT; ct++) base[ct] = log_vs - m[ct];
+            for (int ct = 0; ct < CT; ct++) base[ct] = (exponent - m[ct]) + log_rest;
             if (then) both(cur, nxt, f, base, per_vs, poison, i);
             else weigh(cur, f, base, per_vs, poison, i);
         };
@@ -270,7 +269,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(const AttnArgs A) {
             if (i + 1 < n) step(s1, s0, i + 1);
         }
     }
-    const float down = pow2(-vexp);
+    constexpr float down = 1.0f / (1 << kLift);
 #pragma unroll
     for (int ct = 0; ct < CT; ct++) {
         const float L = row_sum(l[ct]);

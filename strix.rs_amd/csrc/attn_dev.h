@@ -1,6 +1,6 @@
 // Attention of query rows over the paged 8-bit key/value cache.
 //
-//   out[r] = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale * q_r . k_j - running maximum)
+//   out[r] = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale * q_r . k_j - reference)
 //
 // in one pass over the keys.  A row of the kernels is one (token, query head) pair of one sequence and key/value head: all heads
 // of a group read the same keys, so they are rows of one tile.  Everything is computed transposed, S^T = K Q^T and
@@ -10,11 +10,14 @@
 // registers they were formed in.
 //
 // Precision.  Codes are exact in f16, scales stay fp32: a key block's scale multiplies the fp32 products, a value block's the
-// fp32 probabilities.  Queries and probabilities of fp32 calls are split in two f16 terms (hi + lo, 22 bits) and cost two matrix
-// instructions each; one term would leave errors of 2^-12 of a probability, 100 times what an fp32 result should have.
-// bf16 calls use one term (a query's 8 bits are exact, a probability's 11 are 3 more than the result keeps).  Queries
-// are scaled by a power of two of their row's maximum, the value scales by one of the largest in reach, so that neither
-// leaves f16's range; both are undone in fp32.
+// fp32 probabilities.  Queries and weights (probabilities times value scales) of fp32 calls are split in two f16 terms (hi + lo, 22
+// bits) and cost two matrix instructions each; one term would leave errors of 2^-12 of a weight, 100 times what an fp32 result should have.
+// bf16 calls use one term (a query's 8 bits are exact, a weight's 11 are 3 more than the result keeps).
+// f16's range: queries are scaled by a power of two of their row's maximum.  A weight is p_j 2^e u with the value scale's exponent e and
+// u in [1, 2); the reference of the exponentials is the running maximum of score + e (base 2), so a row's largest weight is
+// near 2^5 whatever its probability and scale are, and blocks of far larger values with tiny probabilities (or out of a row's sight) take no
+// bits from the others.  Sums of probabilities take 2^e out again in fp32, which holds while the value scales of a sequence are within
+// 2^100 of each other and above 2^-90: smaller ones are taken for 2^-100 of the largest (2^-90) in these sums.
 #pragma once
 #include "kv_dev.h"
 
@@ -25,10 +28,11 @@ typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 
 constexpr int kSegBlocks = 256;          // blocks whose places and scales are looked up at a time
-constexpr float kLazy = 8.0f;            // the running maximum follows only steps of more than 2^8
+constexpr float kLazy = 8.0f;            // the reference follows only steps of more than 2^8
+constexpr int kLift = 5;                 // weights are 2^kLift times what the reference makes of them: up to 2^14
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMaxPieces = 1024;
-constexpr float kNoMax = -1e30f;         // running maximum of a row that has seen no key
+constexpr float kNoMax = -1e30f;         // reference of a row that has seen no key
 
 struct AttnArgs {
     KvArgs kv;
@@ -36,7 +40,7 @@ struct AttnArgs {
     void* out;
     int64_t ldq, ldo;
     float* part;        // unnormalised sums of pieces, [dim64] each: [rows * q_heads][pieces]
-    float2* part_ml;    // their maxima and sums of probabilities
+    float2* part_ml;    // their references and sums of probabilities
     unsigned* count;    // few rows: finished pieces of each (sequence, head, tile); 0 between launches
     int join;           // few rows: the last workgroup of a row tile to finish joins its pieces
     int tile_rows;
@@ -205,15 +209,12 @@ __device__ __forceinline__ void load_segment(const AttnArgs& A, Segment& seg, in
 }
 template <int WAVES>
 __device__ __forceinline__ float segment_top(const Segment& seg) { return WAVES == 1 ? seg.top[0] : fmaxf(fmaxf(seg.top[0], seg.top[1]), fmaxf(seg.top[2], seg.top[3])); }
-// Exponent that brings value scales up to `top` under 2^6 (times probabilities of up to 2^8 under 2^14).
-__device__ __forceinline__ int value_exponent(float top) {
-    const int e = 5 - (int)((__float_as_uint(top) >> 23) & 255) + 127;
-    return top > 0.f ? min(max(e, -100), 100) : 0;
-}
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }
+__device__ __forceinline__ int exponent_of(float v) { return (int)(__float_as_uint(v) >> 23) - 127; }   // of a v >= 0
+// What value scales below it (0 and NaN among them) lend their exponent from, where the largest one is `top`.
+__device__ __forceinline__ float least_scale(float top) { return pow2(max(exponent_of(top) - 100, -90)); }
 
-// One block of 32 tokens against CT column tiles: scores to probabilities, with the running maximum m and sum l of each row, the
-// sums O rescaled when a maximum moves.  t: [CT][8] scores in base 2 of tokens 4 g + i % 4 + 16 (i / 4) (masked: -inf).
+// References m that the maxima mx of a block's score + e have left behind follow them, and the sums l and o of each row with them.
 template <int CT, int NO>
 __device__ __forceinline__ void rescale(const float (&mx)[CT], float (&m)[CT], float (&l)[CT], v4f (&o)[CT][NO]) {
 #pragma unroll

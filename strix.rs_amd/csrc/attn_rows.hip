@@ -66,7 +66,7 @@ __global__ __launch_bounds__(WAVES * 64, residents(DC, CT)) void attn_rows_kerne
     // every row of the tile sees keys [all_lo, all_hi]: blocks inside need no mask
     const int pos0 = sp.q.len - sp.q.n;
     const int all_hi = pos0 + tile * ROWS / A.group, all_lo = A.window > 0 ? pos0 + min(tile * ROWS + ROWS - 1, rows - 1) / A.group - A.window + 1 : 0;
-    int vexp = 0;
+    float least = 0.f;
     const int tok0 = sp.first + piece * A.piece, tok1 = min(tok0 + A.piece, sp.q.len);
     const int b0 = tok0 / SMX_KV_BLOCK, b1 = (tok1 + SMX_KV_BLOCK - 1) / SMX_KV_BLOCK;
     // a block's bytes are asked for as soon as the registers of the one in front are free: keys behind its scores, values behind
@@ -97,15 +97,7 @@ __global__ __launch_bounds__(WAVES * 64, residents(DC, CT)) void attn_rows_kerne
             fetch(kb, A.kv.k, wave);
             fetch(vb, A.kv.v, wave);
         }
-        const int e = value_exponent(segment_top<WAVES>(seg));
-        if (e != vexp) {
-            const float f = pow2(min(max(e - vexp, -126), 127));
-            for (int ct = 0; ct < CT; ct++)
-#pragma unroll
-                for (int i = 0; i < NO; i++) o[ct][i] *= f;
-            vexp = e;
-        }
-        const float vup = pow2(vexp);
+        least = fmaxf(least, least_scale(segment_top<WAVES>(seg)));
         for (int i = wave; i < n; i += WAVES) {
             v4f sc[CT][2];
 #pragma unroll
@@ -126,7 +118,9 @@ __global__ __launch_bounds__(WAVES * 64, residents(DC, CT)) void attn_rows_kerne
                         for (int k = 0; k < DC * 2; k++) sc[ct][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[k], qf[ct][nt][k], sc[ct][tt], 0, 0, 0);
                 }
             }
-            const float ks = seg.ks[i], vs = seg.vs[i] * vup;
+            const float ks = seg.ks[i], vs = seg.vs[i];
+            const int e = exponent_of(fmaxf(vs, least));
+            const float exponent = (float)e, rest = vs * pow2(kLift - e), inverse = pow2(-e);
             const int next = i + WAVES;
             if (next < n) fetch(kb, A.kv.k, next);
             const int tok = (c0 + i) * SMX_KV_BLOCK;
@@ -145,20 +139,21 @@ __global__ __launch_bounds__(WAVES * 64, residents(DC, CT)) void attn_rows_kerne
                     }
                     mx[ct] = fmaxf(mx[ct], t[ct][j]);
                 }
-                mx[ct] = row_max(mx[ct]);
+                mx[ct] = row_max(mx[ct]) + exponent;
             }
             rescale<CT, NO>(mx, m, l, o);
             v8h pf[CT][NT];
 #pragma unroll
             for (int ct = 0; ct < CT; ct++) {
+                const float base = exponent - m[ct];
                 float p[8], sum = 0.f;
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    const float e2 = __builtin_amdgcn_exp2f(t[ct][j] - m[ct]);
+                    const float e2 = __builtin_amdgcn_exp2f(t[ct][j] + base);
                     sum += e2;
-                    p[j] = edge && t[ct][j] == -INFINITY ? 0.f : e2 * vs;   // (a masked token's value scale may be NaN)
+                    p[j] = edge && t[ct][j] == -INFINITY ? 0.f : e2 * rest;   // (a masked token's value scale may be NaN)
                 }
-                l[ct] += sum;
+                l[ct] = fmaf(sum, inverse, l[ct]);
                 split_prob<NT>(p, pf[ct]);
             }
 #pragma unroll
@@ -176,7 +171,7 @@ __global__ __launch_bounds__(WAVES * 64, residents(DC, CT)) void attn_rows_kerne
         }
     }
     // the four waves' shares of the piece
-    const float down = pow2(-vexp);
+    constexpr float down = 1.0f / (1 << kLift);
 #pragma unroll
     for (int ct = 0; ct < CT; ct++) {
         l[ct] = row_sum(l[ct]);

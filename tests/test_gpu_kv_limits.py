@@ -63,3 +63,68 @@ def test_scale_of_either_sign(accel, pkg, ty, dim, new, scale):
     want = R.attend(cache, table, [length], [new], q, scale)
     # |scores| up to 0.02 * 128 * 3 * sqrt(dim) * |scale|: eight times the tests' 31 at the largest, and so is their rounding
     assert np.abs(got - want).max() <= (8 * TOL[ty] if ty == "f32" else TOL[ty]) * 128 * 0.02
+
+
+def _apart(rng, page, dim, length, big, small, at):
+    """One sequence whose blocks `at` hold values of scale `big` behind scores about 2^-43 of the others' exponentials; the others' scale is
+    `small`.  Channel 0 of every key is +-127, which one large channel of the query turns into the two levels of scores."""
+    cache = _random_cache(rng, page, 1, dim, length)
+    table = R.tables(rng, cache.pages, page, [length])
+    t = np.arange(R.BLOCK)
+    for b in range(-(-length // R.BLOCK)):
+        where = (table[0][b * R.BLOCK // page], 0, b % (page // R.BLOCK))
+        cache.k[where][R.k_byte(cache.dim64, t, 0 * t)] = -127 if b in at else 127
+        cache.ks[where] = np.float32(0.01)
+        cache.vs[where] = np.float32(big if b in at else small)
+        if cache.vs[where] == 0:
+            cache.v[where] = 0
+    return cache, table
+
+
+def _weighed(cache, table, length, new, q, scale):
+    """Per row and head: the largest probability times |value|, what an error is measured by."""
+    k = cache.tokens("k", table[0], 0, length).astype(np.float64)
+    v = np.abs(cache.tokens("v", table[0], 0, length).astype(np.float64)).max(1)
+    out = np.zeros(q.shape[:2])
+    for j in range(new):
+        pos = length - new + j
+        for h in range(q.shape[1]):
+            sc = k[:pos + 1] @ q[j, h].astype(np.float64) * scale
+            p = np.exp(sc - sc.max())
+            out[j, h] = (p * v[:pos + 1]).sum() / p.sum()
+    return out
+
+
+@pytest.mark.parametrize("ty", ["f32", "bf16"])
+@pytest.mark.parametrize("new", [1, 3, 120])
+@pytest.mark.parametrize("big,small", [(0.01, 0.01), (1e4, 0.01), (1e7, 1e-5), (1.0, 1e-20)])
+def test_value_scales_far_apart(accel, pkg, ty, new, big, small):
+    """Blocks of large values whose probabilities are tiny, or that a row does not see, leave the others their bits."""
+    rng = np.random.default_rng(new)
+    dim, length, heads, scale = 64, 900, 2, 0.125
+    cache, table = _apart(rng, 64, dim, length, big, small, (3, 11, 28))
+    q, _ = _queries(rng, "f32", new, heads, dim, 0.3)
+    q[:, :, 0] = 94.0                             # +-127 * 0.01 * 94 / 8 = +-14.9: exponentials 2^-43 apart
+    raw = q if ty == "f32" else R.bf16(q)
+    q = q if ty == "f32" else R.from_bf16(raw)
+    want = R.attend(cache, table, [length], [new], q, scale)
+    got = _attention(accel, pkg, cache, table, [length], [new], raw, ty, scale)
+    err = np.abs(got - want).max(2) / _weighed(cache, table, length, new, q, scale)
+    print(f"{ty} {new} rows, {big:g} beside {small:g}: {err.max():.1e}")
+    assert err.max() <= TOL[ty]
+
+
+@pytest.mark.parametrize("first,then", [(1.0, 1e-28), (1e-28, 1.0), (1e12, 1e-22), (0.0, 1.0), (1.0, 0.0)])
+@pytest.mark.parametrize("new", [1, 70])
+def test_value_scales_change_along_a_long_context(accel, pkg, new, first, then):
+    """Whole sequences (many of them: nothing is split) of more blocks than one look-up holds, whose values change size behind the first."""
+    rng = np.random.default_rng(4)
+    dim, length, nseq, scale = 64, 9000, 600, 0.125
+    cache, one = _apart(rng, 256, dim, length, then, first, range(256, 300))
+    q, raw = _queries(rng, "f32", new, 1, dim, 0.3)
+    want = R.attend(cache, one, [length], [new], q, scale)
+    table = np.repeat(one, nseq, 0)               # (attention only reads: all of them are one sequence)
+    got = _attention(accel, pkg, cache, table, [length] * nseq, [new] * nseq, np.tile(raw, (nseq, 1, 1)), "f32", scale)
+    by = _weighed(cache, one, length, new, q, scale)
+    assert np.array_equal(got.reshape(nseq, new, 1, dim), np.broadcast_to(got[:new], (nseq, new, 1, dim)))
+    assert (np.abs(got[:new] - want).max(2) / by).max() <= TOL["f32"]
