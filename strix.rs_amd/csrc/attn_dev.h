@@ -32,7 +32,7 @@ constexpr float kLazy = 8.0f;            // the reference follows only steps of 
 constexpr int kLift = 5;                 // weights are 2^kLift times what the reference makes of them: up to 2^14
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMaxPieces = 1024;
-constexpr float kNoMax = -1e30f;         // reference of a row that has seen no key
+constexpr float kNoMax = -3.402823466e38f;   // reference of a row that has seen no key: no finite score is below it
 
 struct AttnArgs {
     KvArgs kv;

@@ -128,3 +128,25 @@ def test_value_scales_change_along_a_long_context(accel, pkg, new, first, then):
     by = _weighed(cache, one, length, new, q, scale)
     assert np.array_equal(got.reshape(nseq, new, 1, dim), np.broadcast_to(got[:new], (nseq, new, 1, dim)))
     assert (np.abs(got[:new] - want).max(2) / by).max() <= TOL["f32"]
+
+
+def test_scores_below_every_usual_one(accel, pkg):
+    """All of a row's scores around -1e32: the largest still takes everything."""
+    rng = np.random.default_rng(8)
+    dim, length = 64, 200
+    cache = _random_cache(rng, 32, 1, dim, length)
+    cache.ks[:] = 1e15
+    table = R.tables(rng, cache.pages, 32, [length])
+    t = np.arange(R.BLOCK)
+    for b in range(-(-length // R.BLOCK)):
+        block = cache.k[table[0][b], 0, 0]
+        block[:] = 0
+        block[R.k_byte(64, t, 0 * t)] = rng.integers(-127, 100, R.BLOCK)     # scores of +-127e31 ...
+        block[R.k_byte(64, t, 0 * t + 1)] = -127                             # ... less 254e31
+    cache.k[table[0][0], 0, 0][R.k_byte(64, 0, 0)] = 127                     # the first token's is the largest
+    first = cache.tokens("v", table[0], 0, 1)[0]
+    for new in (1, 90):
+        q = np.zeros((new, 1, dim), np.float32)
+        q[:, :, 0], q[:, :, 1] = 1e16, 2e16
+        got = _attention(accel, pkg, cache, table, [length], [new], q, "f32", 1.0)
+        assert np.abs(got - first).max() <= TOL["f32"] * np.abs(first).max(), new
