@@ -35,6 +35,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(const AttnArgs A) {
     constexpr int KEYS = TB * 2 * KF * 64, TILE = KEYS + TB * NO * 64;   // 16-byte words: keys [block][token / 16][KF][lane], values [block][NO][lane]
     __shared__ Segment seg;
     __shared__ float4 value[kSegBlocks];   // of a block's value scale: exponent e, log2(scale 2^(kLift - e)), 1 / (scale 2^kLift), the scale itself
+    __shared__ float key_top[4];           // largest key scale of each wave's blocks of the segment
     extern __shared__ uint4 stage[];       // [2][TILE]
     const int s = A.listed ? nth_sequence(A, blockIdx.z) : blockIdx.z, piece = blockIdx.y;
     if (s < 0) return;
@@ -59,18 +60,20 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(const AttnArgs A) {
     const int reach = A.window > 0 ? max(pos0 + row0 / A.group - A.window + 1, 0) & ~(SMX_KV_BLOCK - 1) : 0;
     const int tok0 = max(sp.first + piece * A.piece, reach), tok1 = min(min(sp.first + (piece + 1) * A.piece, sp.q.len), last_pos + 1);
     v8h qf[CT][NT][KF];
-    float unit[CT], m[CT], l[CT];
+    float unit[CT], m[CT], l[CT], unit_top = 0.f;
     v4f o[CT][NO];
 #pragma unroll
     for (int ct = 0; ct < CT; ct++) {
         float x[DC][16];
         load_query<DC, BF16>(A, at[ct].live, (int64_t)at[ct].row * A.ldq + (int64_t)at[ct].head * A.kv.dim, x);
         set_query<DC, NT>(A, x, qf[ct], &unit[ct]);
+        unit_top = fmaxf(unit_top, unit[ct]);
         m[ct] = kNoMax;
         l[ct] = 0.f;
 #pragma unroll
         for (int i = 0; i < NO; i++) o[ct][i] = v4f{0.f, 0.f, 0.f, 0.f};
     }
+    unit_top = wave_max(unit_top);
     // this wave's rows: every one sees [all_lo, all_hi]; none sees a token outside [any_lo, any_hi]
     const int wfirst = pos0 + wrow0 / A.group, wlast = pos0 + min(wrow0 + 16 * CT - 1, rows - 1) / A.group;
     const int all_hi = wfirst, all_lo = A.window > 0 ? wlast - A.window + 1 : 0;
@@ -81,7 +84,13 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(const AttnArgs A) {
         const int n = min(kSegBlocks, b1 - c0), tiles = (n + TB - 1) / TB;
         __syncthreads();
         load_segment(A, seg, find_segment(A, s, kvh, c0, n), n);
+        const float top = wave_max((int)threadIdx.x < n ? seg.ks[threadIdx.x] : 0.f);   // (a thread's own)
+        if (lane == 0) key_top[wave] = top;
         __syncthreads();
+        // Scores may be so large that the rounding of the reference is more than what an exponential may exceed it by: they are rounded as it was, on
+        // the way of blocks with masks, where a reference of up to 2^24 takes a product that only the FMA rounds.
+        const bool far = __ballot(fmaxf(fmaxf(key_top[0], key_top[1]), fmaxf(key_top[2], key_top[3])) * unit_top * (32768.0f * 127 * D64) > 0x1p24f) != 0;
+        const int plain_hi = __builtin_amdgcn_readfirstlane(far ? -1 : all_hi);   // blocks up to here need no mask
         least = fmaxf(least, least_scale(segment_top<4>(seg)));
         if ((int)threadIdx.x < n) {
             // (a value scale of 0 stands for codes of 0; a NaN one is for the rows that see a token of the block)
@@ -230,7 +239,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(const AttnArgs A) {
                 return;
             }
             const int tok = (c0 + i) * SMX_KV_BLOCK;
-            const bool edge = tok + SMX_KV_BLOCK - 1 > all_hi || tok < all_lo;
+            const bool edge = tok + SMX_KV_BLOCK - 1 > plain_hi || tok < all_lo;
             const float ks = seg.ks[i];
             const float4 vs = value[i];
             const float exponent = vs.x, log_rest = vs.y, per_vs = vs.z, poison = vs.w == vs.w ? 0.f : vs.w;

@@ -109,6 +109,12 @@ __device__ __forceinline__ float row_max(float v) {
     s = swap16(fmaxf(s.x, s.y));
     return fmaxf(s.x, s.y);
 }
+__device__ __forceinline__ float wave_max(float v) {
+    v = row_max(v);
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) v = fmaxf(v, __shfl_xor(v, o));
+    return v;
+}
 __device__ __forceinline__ float row_sum(float v) {
     float2 s = swap32(v);
     s = swap16(s.x + s.y);
@@ -202,9 +208,7 @@ __device__ __forceinline__ void load_segment(const AttnArgs& A, Segment& seg, in
         seg.vs[threadIdx.x] = v;
         top = fmaxf(v, 0.f);   // (a NaN scale does not count)
     }
-    top = row_max(top);
-#pragma unroll
-    for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
+    top = wave_max(top);
     if ((threadIdx.x & 63) == 0) seg.top[threadIdx.x >> 6] = top;
 }
 template <int WAVES>

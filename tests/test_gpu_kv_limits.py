@@ -150,3 +150,30 @@ def test_scores_below_every_usual_one(accel, pkg):
         q[:, :, 0], q[:, :, 1] = 1e16, 2e16
         got = _attention(accel, pkg, cache, table, [length], [new], q, "f32", 1.0)
         assert np.abs(got - first).max() <= TOL["f32"] * np.abs(first).max(), new
+
+
+@pytest.mark.parametrize("ty", ["f32", "bf16"])
+@pytest.mark.parametrize("size", [1e6, 1e10, 1e32])
+@pytest.mark.parametrize("dim,sign", [(64, 1), (64, -1), (128, 1), (256, -1)])
+def test_scores_of_every_size(accel, pkg, ty, size, dim, sign):
+    """Scores of which fp32 keeps no fraction, of both signs: one token stands out for every row and takes everything."""
+    rng = np.random.default_rng(9)
+    length, best = 300, 77
+    cache = _random_cache(rng, 32, 1, dim, length)
+    cache.ks[:], cache.vs[:] = 0.5, 0.01
+    table = R.tables(rng, cache.pages, 32, [length])
+    t = np.arange(R.BLOCK)
+    for b in range(-(-length // R.BLOCK)):
+        block = cache.k[table[0][b], 0, 0]
+        block[:] = 0
+        block[R.k_byte(cache.dim64, t, 0 * t)] = rng.integers(-100, 100, R.BLOCK)
+    cache.k[table[0][best // 32], 0, 0][R.k_byte(cache.dim64, best % 32, 0)] = 127 * sign
+    want = cache.tokens("v", table[0], 0, best + 1)[best]
+    for new in (1, 200):
+        q = np.zeros((new, 1, dim), np.float32)
+        q[:, :, 0] = size / 64.0
+        raw = q if ty == "f32" else R.bf16(q)
+        got = _attention(accel, pkg, cache, table, [length], [new], raw, ty, float(sign))
+        seen = np.arange(length - new, length) >= best       # (earlier rows of the chunk: some other token)
+        assert np.isfinite(got).all()
+        assert np.abs(got[seen] - want).max() <= TOL[ty] * np.abs(want).max(), new
