@@ -279,7 +279,9 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs A) {
         g[j].fetch(keys ? A.k : A.v, (int64_t)(br.row + tok[j]) * (keys ? A.ldk : A.ldv) + (int64_t)head * a.dim);
         if (nth[j] * W < rot >> 1) g[j].fetch_turn(A.rope + (int64_t)min(br.blk * SMX_KV_BLOCK + tok[j], A.n_pos - 1) * (rot >> 1), nth[j]);
     }
-    const int64_t bi = kv_block(a, br.s, head, br.blk);
+    const int page = kv_page(a, br.s, br.blk);
+    if (page < 0 || page >= a.pages) return;   // (the same for the workgroup) clamped, the block would be one of another sequence's
+    const int64_t bi = kv_place(a, page, head, br.blk);
     float* sp = (keys ? a.ks : a.vs) + bi;
     const float before = t0 > 0 ? *sp : 0.0f;
     for (int u = tid; u < 2 * a.dim64; u += 256) ((uint4*)image)[u] = make_uint4(0, 0, 0, 0);

@@ -38,11 +38,13 @@ __device__ __forceinline__ KvSeq kv_seq(const KvArgs& a, int s) {
     }
     return q;
 }
-// Index of a head's block `blk` (of SMX_KV_BLOCK tokens) of sequence s among all blocks of the cache.
+// The page that the table names for block `blk` (of SMX_KV_BLOCK tokens) of sequence s: any number at all.
+__device__ __forceinline__ int kv_page(const KvArgs& a, int s, int blk) { return a.table[(int64_t)s * a.table_ld + min(blk / a.page_blocks, a.table_ld - 1)]; }
+// Index of a head's block `blk` of a page of the cache among all blocks.
+__device__ __forceinline__ int64_t kv_place(const KvArgs& a, int page, int head, int blk) { return ((int64_t)page * a.kv_heads + head) * a.page_blocks + blk % a.page_blocks; }
+// The same of sequence s, for reading: page numbers outside the cache are clamped into it.
 __device__ __forceinline__ int64_t kv_block(const KvArgs& a, int s, int head, int blk) {
-    const int p = blk / a.page_blocks;
-    const int page = min(max(a.table[(int64_t)s * a.table_ld + min(p, a.table_ld - 1)], 0), a.pages - 1);
-    return ((int64_t)page * a.kv_heads + head) * a.page_blocks + (blk - p * a.page_blocks);
+    return kv_place(a, min(max(kv_page(a, s, blk), 0), a.pages - 1), head, blk);
 }
 // Byte of (token, channel) inside a block's keys / values.
 __device__ __forceinline__ int kv_k_byte(int dim64, int t, int d) {

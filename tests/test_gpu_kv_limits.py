@@ -177,3 +177,44 @@ def test_scores_of_every_size(accel, pkg, ty, size, dim, sign):
         seen = np.arange(length - new, length) >= best       # (earlier rows of the chunk: some other token)
         assert np.isfinite(got).all()
         assert np.abs(got[seen] - want).max() <= TOL[ty] * np.abs(want).max(), new
+
+
+@pytest.mark.parametrize("ty", ["f32", "bf16"])
+def test_nothing_is_stored_outside_the_cache(accel, pkg, ty):
+    """Page numbers that name no page: their tokens are left out, every other byte of the cache, of the read-back and of the queries is as it
+    was or as the definition says."""
+    rng = np.random.default_rng(12)
+    kv, heads, dim, page, pages = 2, 4, 64, 32, 6
+    lens, new = [70, 40, 33, 65], [70, 40, 2, 1]
+    table = np.array([[4, -1, 1], [-7, 5, -1], [6, 3, 0], [99, 2 ** 31 - 1, -2 ** 31]], np.int32)
+    rows = sum(new)
+    cache = R.Cache(pages, page, kv, dim, seed=2)
+    cache.ks[:], cache.vs[:] = 0.01, 0.02
+    want = [x.copy() for x in (cache.k, cache.v, cache.ks, cache.vs)]
+    k, raw_k = _queries(rng, ty, rows, kv, dim)
+    v, raw_v = _queries(rng, ty, rows, kv, dim)
+    # the definition, token by token of the pages that exist: a sequence's own table with spare pages behind the cache for the others
+    big = R.Cache(pages + 12, page, kv, dim, seed=2)
+    for a, b in ((big.k, cache.k), (big.v, cache.v), (big.ks, cache.ks), (big.vs, cache.vs)):
+        a[:] = 0
+        a[:pages] = b
+    own = np.where((table >= 0) & (table < pages), table, pages + np.arange(12).reshape(4, 3)).astype(np.int32)
+    R.append(big, own, [a - b for a, b in zip(lens, new)], new, k, v)
+    want = [x[:pages] for x in (big.k, big.v, big.ks, big.vs)]
+    guard = 4096
+    with R.Dev(accel) as dev:
+        d = R.OnDevice(pkg, dev, cache)
+        held, planes = [], []
+        for x in (cache.k, cache.v, cache.ks, cache.vs):     # planes with guards on both sides
+            raw = np.concatenate([np.full(guard, 0xA5, np.uint8), np.frombuffer(x.tobytes(), np.uint8), np.full(guard, 0xA5, np.uint8)])
+            held.append((dev.put(raw), raw.size))
+            planes.append(held[-1][0] + guard)
+        handle = pkg.KvCache(pages, page, kv, dim, *planes)
+        batch = d.batch(table, lens, new)
+        accel.kv_append_dev(handle, batch, dev.put(raw_k), dev.put(raw_v), dtype=_dtype(pkg, ty))
+        for (p, n), w in zip(held, want):
+            got = dev.get(p, n, np.uint8)
+            assert (got[:guard] == 0xA5).all() and (got[n - guard:] == 0xA5).all()
+            body = np.frombuffer(got[guard:n - guard].tobytes(), w.dtype).reshape(w.shape)
+            same = (body == w) | ((body != body) & (w != w))
+            assert same.all(), np.argwhere(~same)[:4]
