@@ -21,21 +21,26 @@ struct KvArgs {
     int nseq, rows, max_rows, max_len;
 };
 
-// One sequence of the batch: its rows [row, row + n) and the tokens [0, len) it holds; row j is the token len - n + j.
+// One sequence of the batch as far as it is within the call's sizes: its rows [row, row + n) and the tokens [0, len) it holds; row j is the
+// token len - n + j.  What is beyond rows, max_rows or max_len are a sequence's last rows, and go with their tokens: the others keep
+// their positions.
 struct KvSeq {
     int row, n, len;
 };
 __device__ __forceinline__ KvSeq kv_seq(const KvArgs& a, int s) {
     KvSeq q;
-    q.len = min(max(a.len[s], 0), a.max_len);
+    q.len = max(a.len[s], 0);
+    q.row = s;
+    q.n = 1;
     if (a.row0) {
-        const int r0 = min(max(a.row0[s], 0), a.rows), r1 = min(max(a.row0[s + 1], r0), a.rows);
-        q.row = r0;
-        q.n = min(r1 - r0, a.max_rows);
-    } else {
-        q.row = s;
-        q.n = 1;
+        q.row = min(max(a.row0[s], 0), a.rows);
+        const int all = max(a.row0[s + 1], q.row) - q.row;
+        q.n = min(all, min(a.rows - q.row, a.max_rows));
+        q.len = max(q.len - (all - q.n), 0);
     }
+    const int over = max(q.len - a.max_len, 0);
+    q.n = max(q.n - over, 0);
+    q.len -= over;
     return q;
 }
 // The page that the table names for block `blk` (of SMX_KV_BLOCK tokens) of sequence s: any number at all.

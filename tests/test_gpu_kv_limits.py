@@ -218,3 +218,66 @@ def test_nothing_is_stored_outside_the_cache(accel, pkg, ty):
             body = np.frombuffer(got[guard:n - guard].tobytes(), w.dtype).reshape(w.shape)
             same = (body == w) | ((body != body) & (w != w))
             assert same.all(), np.argwhere(~same)[:4]
+
+
+def _rows_of(x, ranges):
+    return np.concatenate([x[a:b] for a, b in ranges])
+
+
+@pytest.mark.parametrize("new", [[1, 1], [5, 3], [70, 40]])
+@pytest.mark.parametrize("how", ["max_len", "max_rows", "rows"])
+def test_rows_beyond_the_call_are_left_out(accel, pkg, new, how):
+    """Arrays that name more tokens or rows than the call's sizes: the rows within them are at their own positions, the others are neither stored
+    nor attended to, and what the sequences held stays."""
+    if how == "max_rows" and max(new) == 1:
+        pytest.skip("a row each")
+    rng = np.random.default_rng(sum(new))
+    kv, heads, dim, page = 2, 4, 64, 32
+    old = [100, 37]
+    lens = [a + b for a, b in zip(old, new)]
+    rows = sum(new)
+    cache = R.Cache(14, page, kv, dim, seed=5)
+    table = R.tables(rng, 14, page, lens)
+    R.append(cache, table, [0, 0], old, *(rng.standard_normal((sum(old), kv, dim)).astype(np.float32) for _ in range(2)))
+    k, v = (rng.standard_normal((rows, kv, dim)).astype(np.float32) for _ in range(2))
+    q, _ = _queries(rng, "f32", rows, heads, dim)
+    # what the call's sizes leave of each sequence's rows
+    left = {"max_len": [max(0, new[0] - 1), new[1]], "max_rows": [min(n, max(new) - 2) for n in new], "rows": [new[0], new[1] - 1]}[how]
+    limits = {"max_len": dict(max_len=lens[0] - 1), "max_rows": {}, "rows": {}}[how]
+    rope = R.rope_table(max(lens), dim)
+    ranges = [(0, left[0]), (new[0], new[0] + left[1])]
+    held = [a + b for a, b in zip(old, left)]
+    pos = np.concatenate([np.arange(a, b) for a, b in zip(old, held)])
+    with R.Dev(accel) as dev:
+        d = R.OnDevice(pkg, dev, cache)
+        b = d.batch(table, lens, new, always_row0=how != "max_len" or max(new) > 1, **limits)
+        if how == "max_rows":
+            b.max_rows = max(new) - 2
+        elif how == "rows":
+            b.rows -= 1
+            b.max_rows = min(b.max_rows, b.rows)
+        out, back = dev.put(np.full(q.shape, 7, np.float32)), [dev.put(np.full(k.shape, 7, np.float32)) for _ in range(2)]
+        accel.kv_append_dev(d.handle, b, dev.put(k), dev.put(v), rope=pkg.Rope(dev.put(rope), rope.shape[0], dim))
+        R.append(cache, table, old, left, R.rotate(_rows_of(k, ranges), rope, pos, dim, False), _rows_of(v, ranges))
+        got = d.planes()
+        for a, w in zip(got[2:], (cache.ks, cache.vs)):
+            assert np.array_equal(a, w, equal_nan=True)
+        host = R.Cache(1, page, kv, dim)
+        host.k, host.v, host.ks, host.vs = got
+        for s, n in enumerate(held):
+            for h in range(kv):
+                for w in "kv":
+                    assert np.array_equal(host.tokens(w, table[s], h, n), cache.tokens(w, table[s], h, n)), (s, h, w)
+        accel.attn_dev(d.handle, b, dev.put(q), heads, dim ** -0.5, out)
+        accel.kv_read_dev(d.handle, b, *back)
+        y, back = dev.get(out, q.shape), [dev.get(p, k.shape) for p in back]
+    want = R.attend(cache, table, held, left, _rows_of(q, ranges), dim ** -0.5)
+    assert np.abs(_rows_of(y, ranges) - want).max(initial=0) <= TOL["f32"] * 5
+    beyond = np.setdiff1d(np.arange(rows), np.concatenate([np.arange(*r) for r in ranges]))
+    assert (y[beyond] == 7).all()
+    for x, w in zip(back, "kv"):
+        assert (x[beyond] == 7).all()
+        r = 0
+        for s, (o, n) in enumerate(zip(old, held)):
+            for h in range(kv):
+                assert np.array_equal(x[ranges[s][0]:ranges[s][1], h], cache.tokens(w, table[s], h, n)[o:])
