@@ -279,9 +279,8 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs A) {
         g[j].fetch(keys ? A.k : A.v, (int64_t)(br.row + tok[j]) * (keys ? A.ldk : A.ldv) + (int64_t)head * a.dim);
         if (nth[j] * W < rot >> 1) g[j].fetch_turn(A.rope + (int64_t)min(br.blk * SMX_KV_BLOCK + tok[j], A.n_pos - 1) * (rot >> 1), nth[j]);
     }
-    const int page = kv_page(a, br.s, br.blk);
-    if (page < 0 || page >= a.pages) return;   // (the same for the workgroup) clamped, the block would be one of another sequence's
-    const int64_t bi = kv_place(a, page, head, br.blk);
+    const KvPlace at = kv_place(a, br.s, head, br.blk);
+    const int64_t bi = at.block;
     float* sp = (keys ? a.ks : a.vs) + bi;
     const float before = t0 > 0 ? *sp : 0.0f;
     for (int u = tid; u < 2 * a.dim64; u += 256) ((uint4*)image)[u] = make_uint4(0, 0, 0, 0);
@@ -298,6 +297,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs A) {
     for (int o = 1; o < 64; o <<= 1) most = max(most, (unsigned)__shfl_xor((int)most, o));
     if ((tid & 63) == 0) red[tid >> 6] = most;
     __syncthreads();   // (every thread has read the old scale, too)
+    if (at.page < 0 || at.page >= a.pages) return;   // (the same for the workgroup) the clamped one is another sequence's
     most = max(max(red[0], red[1]), max(red[2], red[3]));
     const float top = __uint_as_float(most);
     const float fresh = most >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : top >= 0x1p-96f ? top / 127.0f : 0.0f;

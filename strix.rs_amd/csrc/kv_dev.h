@@ -28,29 +28,29 @@ struct KvSeq {
     int row, n, len;
 };
 __device__ __forceinline__ KvSeq kv_seq(const KvArgs& a, int s) {
+    const int len = a.len[s];
+    int r0 = s, r1 = s + 1;   // (without row0 rows is nseq and max_rows 1)
+    if (a.row0) { r0 = a.row0[s]; r1 = a.row0[s + 1]; }
     KvSeq q;
-    q.len = max(a.len[s], 0);
-    q.row = s;
-    q.n = 1;
-    if (a.row0) {
-        q.row = min(max(a.row0[s], 0), a.rows);
-        const int all = max(a.row0[s + 1], q.row) - q.row;
-        q.n = min(all, min(a.rows - q.row, a.max_rows));
-        q.len = max(q.len - (all - q.n), 0);
-    }
+    q.row = min(max(r0, 0), a.rows);
+    const int all = max(r1, q.row) - q.row, kept = min(all, min(a.rows - q.row, a.max_rows));
+    q.len = max(max(len, 0) - (all - kept), 0);
     const int over = max(q.len - a.max_len, 0);
-    q.n = max(q.n - over, 0);
+    q.n = max(kept - over, 0);
     q.len -= over;
     return q;
 }
-// The page that the table names for block `blk` (of SMX_KV_BLOCK tokens) of sequence s: any number at all.
-__device__ __forceinline__ int kv_page(const KvArgs& a, int s, int blk) { return a.table[(int64_t)s * a.table_ld + min(blk / a.page_blocks, a.table_ld - 1)]; }
-// Index of a head's block `blk` of a page of the cache among all blocks.
-__device__ __forceinline__ int64_t kv_place(const KvArgs& a, int page, int head, int blk) { return ((int64_t)page * a.kv_heads + head) * a.page_blocks + blk % a.page_blocks; }
-// The same of sequence s, for reading: page numbers outside the cache are clamped into it.
-__device__ __forceinline__ int64_t kv_block(const KvArgs& a, int s, int head, int blk) {
-    return kv_place(a, min(max(kv_page(a, s, blk), 0), a.pages - 1), head, blk);
+// Where a head's block `blk` (of SMX_KV_BLOCK tokens) of sequence s is: the page that the table names for it (any number at all), and its index
+// among all blocks of the cache, with page numbers outside the cache clamped into it.
+struct KvPlace {
+    int page;
+    int64_t block;
+};
+__device__ __forceinline__ KvPlace kv_place(const KvArgs& a, int s, int head, int blk) {
+    const int p = blk / a.page_blocks, page = a.table[(int64_t)s * a.table_ld + min(p, a.table_ld - 1)];
+    return {page, ((int64_t)min(max(page, 0), a.pages - 1) * a.kv_heads + head) * a.page_blocks + (blk - p * a.page_blocks)};
 }
+__device__ __forceinline__ int64_t kv_block(const KvArgs& a, int s, int head, int blk) { return kv_place(a, s, head, blk).block; }
 // Byte of (token, channel) inside a block's keys / values.
 __device__ __forceinline__ int kv_k_byte(int dim64, int t, int d) {
     return ((t >> 4) * (dim64 >> 6) + (d >> 6)) * 1024 + ((d >> 4) & 3) * 256 + (t & 15) * 16 + (d & 15);
