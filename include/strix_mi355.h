@@ -320,7 +320,8 @@ int smx_kv_read_dev(smx_ctx* ctx, const smx_kv_cache* cache, const smx_kv_batch*
  * fp32 rows are computed to fp32 accuracy (queries and probabilities as two f16 terms each on the matrix cores; errors are relative
  * to the row's largest probability times value, as long as the value scales of a sequence are above 2^-90 and within 2^100 of each
  * other), bf16 rows with one f16 term; statistics and sums are fp32.  A row's result depends on its own sequence and on the sizes of
- * the call (nseq, rows, max_rows, max_len, which set how a long sequence is split), not on the other sequences.  Capturable. */
+ * the call (nseq, rows, max_rows, max_len, which set how a long sequence is split), not on the other sequences.  Capturable.
+ * SMX_ERR_LIMIT, here as for the append: more than 65535 sequences, 2^24 rows or 2^28 tokens, or rows * q_heads of 2^31 and more. */
 int smx_attn_dev(smx_ctx* ctx, const smx_kv_cache* cache, const smx_kv_batch* batch, int type, const void* q_dev, size_t ldq,
                  size_t q_heads, float scale, size_t window, void* out_dev, size_t ldo);
 

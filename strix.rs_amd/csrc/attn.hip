@@ -505,6 +505,8 @@ extern "C" int smx_attn_dev(smx_ctx* c, const smx_kv_cache* cache, const smx_kv_
     const size_t width = q_heads * cache->head_dim;
     if (ldq < width || ldo < width) return fail(c, SMX_ERR_ARG, "attn_dev: rows of %zu elements, ldq %zu, ldo %zu", width, ldq, ldo);
     if (batch->nseq == 0 || batch->rows == 0) return SMX_OK;
+    // (rows of a head's group are counted in 32 bits)
+    if (batch->rows * q_heads >= (size_t(1) << 31)) return fail(c, SMX_ERR_LIMIT, "attn_dev: %zu rows of %zu query heads (2^31 in all)", batch->rows, q_heads);
     if (!q || !out) return fail(c, SMX_ERR_ARG, "attn_dev: null queries or result");
     const bool bf16 = type == SMX_TYPE_BF16;
     A.q = q; A.out = out; A.ldq = (int64_t)ldq; A.ldo = (int64_t)ldo;

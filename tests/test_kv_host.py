@@ -33,3 +33,17 @@ a.attn_dev(cache, b, room, HEADS, 1.0, room)
 a.kv_append_dev(cache, b, room, room)
 a.kv_read_dev(cache, b, room, room)
 """)
+
+
+def test_more_rows_than_are_counted(run):   # noqa: F811
+    """Rows times heads of 2^31 and more: refused by the attention as by the append."""
+    run(SETUP + """
+one = pkg.KvCache(64, 64, 1, 2, room, room, room, room)
+for rows, heads in ((1 << 24, 128), (1 << 23, 256), (1 << 20, 2048), (1 << 24, 65535)):
+    b = batch(1, rows, rows)
+    refused(lambda: a.attn_dev(one, b, room, heads, 1.0, room), -3)
+    refused(lambda: a.kv_append_dev(one, b, room, room, q=room, q_heads=heads, q_out=room), -3)
+launches = F.fake_launches()
+a.attn_dev(one, batch(1, 1 << 16, 1 << 16, 64), room, 1, 1.0, room)
+assert F.fake_launches() > launches
+""")
