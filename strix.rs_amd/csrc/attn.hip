@@ -307,9 +307,10 @@ __global__ __launch_bounds__(256) void attn_join_few_kernel(const AttnArgs A) {
     const int quads = A.kv.dim64 >> 2, nth = threadIdx.x / quads, units = 256 / quads, d = (threadIdx.x - nth * quads) * 4;   // quads: 16, 32, 48 or 64
     const int unit = blockIdx.x * units + nth, row = unit / A.q_heads, head = unit - row * A.q_heads;
     if (nth >= units || row >= A.kv.rows) return;
-    const Span sp = seq_span(A, seq_of_row(A.kv, row));
+    const int s = seq_of_row(A.kv, row);
+    const Span sp = seq_span(A, s);
     if (sp.pieces <= 1 || row >= sp.q.row + sp.q.n) return;
-    const int64_t at = (int64_t)unit * A.pieces;
+    const int64_t at = sums_of(A, s, sp.q, row, head) * A.pieces;
     float M = kNoMax, L = 0.f;
 #pragma unroll 4
     for (int i = 0; i < sp.pieces; i++) M = fmaxf(M, A.part_ml[at + i].x);
@@ -334,9 +335,10 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs A) {
     __shared__ float factor[kMaxPieces], red[2][4];
     __shared__ v4f sums[256];
     const int row = blockIdx.x, head = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const Span sp = seq_span(A, seq_of_row(A.kv, row));
+    const int s = seq_of_row(A.kv, row);
+    const Span sp = seq_span(A, s);
     if (sp.pieces <= 1 || row >= sp.q.row + sp.q.n) return;
-    const int64_t at = ((int64_t)row * A.q_heads + head) * A.pieces;
+    const int64_t at = sums_of(A, s, sp.q, row, head) * A.pieces;
     float M = kNoMax;
     for (int i = tid; i < sp.pieces; i += 256) M = fmaxf(M, A.part_ml[at + i].x);
 #pragma unroll
@@ -440,17 +442,21 @@ int attend(smx_ctx* c, AttnArgs A, size_t nseq, size_t rows, size_t reach, bool 
     size_t split = std::max<size_t>(1, cus / groups);
     if (span <= kWhole) split = 1;
     else if (2 * cus / groups > split && span / (2 * cus / groups) >= (few ? kWorthFew : kWorthMany)) split = 2 * cus / groups;
-    // and no piece is longer than kLongest to 2 kLongest, as far as there is room for the pieces' sums
-    const size_t outputs = (size_t)A.kv.rows * A.q_heads, each = (size_t)A.kv.dim64 * 4 + 8;
-    split = std::max(split, std::min<size_t>(span * A.kv.dim64 / 128 / kLongest, kMostSums / (outputs * each)));
-    split = std::min<size_t>(split, kMaxPieces);
+    // and no piece is longer than kLongest to 2 kLongest; all of it as far as there is room for the pieces' sums.  Each of the call's rows has a
+    // place for its own; of few rows beside many it is each that a sequence may have (one chunk of 8192 rows and a decode step of 32 heads of
+    // 128 channels at 100000 tokens: 4.4 GB the first way, 17 MB the second)
+    const size_t outputs = (size_t)A.kv.rows * A.q_heads, each = (size_t)A.kv.dim64 * 4 + 8, by_seq = all * A.kv.kv_heads * top;
+    A.few_rows = few && by_seq < outputs ? (int)top : 0;
+    const size_t kept = A.few_rows ? by_seq : outputs;
+    split = std::max(split, span * A.kv.dim64 / 128 / kLongest);
+    split = std::min({split, std::max<size_t>(1, kMostSums / (kept * each)), (size_t)kMaxPieces});
     const size_t places = cus * rows_residents(A.kv.dim64, A.tile_rows);
     A.lone = few && groups > places && (span <= kLone || (A.window > 0 && 4 * groups >= 5 * places && groups <= 2 * places && span <= kLoneWindow));
     const size_t piece = std::max<size_t>(((span + split - 1) / split + 127) & ~size_t(127), 128);
     A.piece = (int)std::min<size_t>(piece, size_t(1) << 30);
     A.pieces = (int)std::max<size_t>((reach + piece - 1) / piece, 1);
     if (A.pieces > 1) {
-        const size_t n = outputs * (size_t)A.pieces;
+        const size_t n = kept * (size_t)A.pieces;
         if ((rc = ensure(c, c->work, n * each)) != SMX_OK) return rc;
         A.part = (float*)c->work.p;
         A.part_ml = (float2*)(A.part + n * A.kv.dim64);

@@ -39,11 +39,12 @@ struct AttnArgs {
     const void* q;
     void* out;
     int64_t ldq, ldo;
-    float* part;        // unnormalised sums of pieces, [dim64] each: [rows * q_heads][pieces]
+    float* part;        // unnormalised sums of pieces, [dim64] each: [sums_of()][pieces]
     float2* part_ml;    // their references and sums of probabilities
     unsigned* count;    // few rows: finished pieces of each (sequence, head, tile); 0 between launches
     int join;           // few rows: the last workgroup of a row tile to finish joins its pieces
     int tile_rows;
+    int few_rows;       // places that each sequence's rows of a key/value head have for their sums; 0: each of the call's rows has one (see sums_of)
     int above, upto;    // sequences of more than `above` and up to `upto` rows of a key/value head are this launch's
     int listed;         // many rows: workgroups z serve the z-th of the sequences that are this launch's
     int q_heads, group, window;
@@ -263,6 +264,15 @@ __device__ __forceinline__ RowAt row_at(const AttnArgs& A, const KvSeq& q, int k
     x.pos = q.len - q.n + tok;
     return x;
 }
+// Where the sums of a row's pieces are, in units of all its pieces; r: the row among its sequence's of the key/value head.  A launch for few
+// rows goes by its sequences where the call's other rows, a prompt chunk beside decode steps say, are many times its own.
+__device__ __forceinline__ int64_t sums_of(const AttnArgs& A, int s, int kvh, int r, int row, int head) {
+    return A.few_rows ? ((int64_t)s * A.kv.kv_heads + kvh) * A.few_rows + r : (int64_t)row * A.q_heads + head;
+}
+__device__ __forceinline__ int64_t sums_of(const AttnArgs& A, int s, const KvSeq& q, int row, int head) {
+    const int kvh = head / A.group;
+    return sums_of(A, s, kvh, (row - q.row) * A.group + (head - kvh * A.group), row, head);
+}
 // 4 channels d.. of one row of the result
 template <bool BF16>
 __device__ __forceinline__ void store_out(const AttnArgs& A, const RowAt& r, int d, v4f o) {
@@ -276,7 +286,7 @@ __device__ __forceinline__ void store_out(const AttnArgs& A, const RowAt& r, int
             if (d + i < A.kv.dim) store_elem<BF16>(A.out, at + i, o[i]);
     }
 }
-// A piece's share of one row: the result itself where the sequence is one piece, else sums for attn_join_kernel.
+// A piece's share of one row (of many): the result itself where the sequence is one piece, else sums for attn_join_kernel.
 template <bool BF16>
 __device__ __forceinline__ void put_row(const AttnArgs& A, const RowAt& r, int piece, int pieces, int d, v4f o, float m, float l, bool first) {
     if (!r.live) return;

@@ -195,7 +195,7 @@ __global__ __launch_bounds__(WAVES * 64, residents(DC, CT)) void attn_rows_kerne
         for (int v = 0; v < WAVES; v++) L += wl[v][r] * __builtin_amdgcn_exp2f(wm[v][r] - M);
         __syncthreads();
         if (!at[ct].live) continue;
-        const int64_t mine = ((int64_t)at[ct].row * A.q_heads + at[ct].head) * A.pieces + piece;
+        const int64_t mine = sums_of(A, s, kvh, tile * ROWS + r, at[ct].row, at[ct].head) * A.pieces + piece;
         if (sp.pieces > 1 && wave == 0 && g == 0) {
             give(&A.part_ml[mine].x, M);
             give(&A.part_ml[mine].y, L);
@@ -236,7 +236,7 @@ __global__ __launch_bounds__(WAVES * 64, residents(DC, CT)) void attn_rows_kerne
         float2 ml = make_float2(kNoMax, 0.f);
         if (i < sp.pieces) {
             const RowAt x = row_at(A, sp.q, kvh, tile * ROWS + r);
-            const float2* from = A.part_ml + ((int64_t)x.row * A.q_heads + x.head) * A.pieces + i;
+            const float2* from = A.part_ml + sums_of(A, s, kvh, tile * ROWS + r, x.row, x.head) * A.pieces + i;
             ml = make_float2(take(&from->x), take(&from->y));
         }
         const float M = row16_max(ml.x);
@@ -248,7 +248,7 @@ __global__ __launch_bounds__(WAVES * 64, residents(DC, CT)) void attn_rows_kerne
     const int gr = threadIdx.x / QUADS, d = (threadIdx.x - gr * QUADS) * 4;
     for (int r = gr; r < live && gr < GROUPS; r += GROUPS) {
         const RowAt x = row_at(A, sp.q, kvh, tile * ROWS + r);
-        const float* from = A.part + ((int64_t)x.row * A.q_heads + x.head) * A.pieces * D64 + d;
+        const float* from = A.part + sums_of(A, s, kvh, tile * ROWS + r, x.row, x.head) * A.pieces * D64 + d;
         v4f acc = v4f{0.f, 0.f, 0.f, 0.f};
         float L = 0.f;
         for (int i = 0; i < sp.pieces; i += 4) {

@@ -92,6 +92,7 @@ bool g_keep_inbound = false;
 int g_slow_us = 0;
 size_t g_host_limit = SIZE_MAX, g_host_live = 0;
 std::map<void*, size_t> g_host;
+std::map<void*, size_t> g_device;
 std::atomic<int> g_host_refused{0}, g_launches{0}, g_failed_launches{0};
 std::vector<unsigned> g_host_flags;
 thread_local hipError_t t_last = hipSuccess;
@@ -127,6 +128,12 @@ size_t fake_inbound(char* out, size_t cap) {   // what host-to-device copy comma
 void fake_host_limit(size_t bytes) { g_host_limit = bytes; }   // a larger pinned allocation is refused
 int fake_host_refused() { return g_host_refused; }
 size_t fake_host_live() { return g_host_live; }
+size_t fake_device_live() {
+    std::lock_guard<std::mutex> l(g_mu);
+    size_t n = 0;
+    for (auto& d : g_device) n += d.second;
+    return n;
+}
 int fake_host_noncoherent() {   // pinned allocations that did not ask for coherent memory
     std::lock_guard<std::mutex> l(g_mu);
     int n = 0;
@@ -250,9 +257,15 @@ hipError_t hipMalloc(void** p, size_t n) {
     if (!w) return done(hipErrorOutOfMemory);
     for (size_t i = 0; n <= kGigabyte && i < words; i++) w[i] = (unsigned)i;
     *p = w;
+    std::lock_guard<std::mutex> l(g_mu);
+    g_device[w] = n;
     return hipSuccess;
 }
 hipError_t hipFree(void* p) {
+    {
+        std::lock_guard<std::mutex> l(g_mu);
+        g_device.erase(p);
+    }
     std::free(p);
     return hipSuccess;
 }

@@ -281,3 +281,24 @@ def test_rows_beyond_the_call_are_left_out(accel, pkg, new, how):
         for s, (o, n) in enumerate(zip(old, held)):
             for h in range(kv):
                 assert np.array_equal(x[ranges[s][0]:ranges[s][1], h], cache.tokens(w, table[s], h, n)[o:])
+
+
+@pytest.mark.parametrize("ty,dim,kv,group,few,chunk", [("f32", 64, 1, 1, [1], 700), ("f32", 128, 2, 4, [1, 1, 0, 1], 300), ("bf16", 64, 1, 8, [1, 5], 200),
+                                                       ("f32", 64, 2, 2, [1] * 40, 90), ("bf16", 256, 1, 2, [1, 2, 30], 120)])
+def test_split_contexts_of_decode_steps_beside_chunks(accel, pkg, ty, dim, kv, group, few, chunk):
+    """Sequences of few rows and chunks of many in one call, at contexts that are split: both launches' sums find their rows again, and a second
+    call on the same context finds its own."""
+    rng = np.random.default_rng(dim + chunk)
+    heads, page, length = kv * group, 64, 3000
+    cache = _random_cache(rng, page, kv, dim, 4 * length)
+    new = few[:len(few) // 2] + [chunk] + few[len(few) // 2:]
+    lens = [length - int(x) for x in rng.integers(0, length // 2, len(new))]
+    pages = rng.permutation(cache.pages)
+    table = np.stack([np.roll(pages, i)[:-(-length // page)] for i in range(len(new))]).astype(np.int32)   # (they may share pages: nothing is stored)
+    q, raw = _queries(rng, ty, sum(new), heads, dim)
+    want = R.attend(cache, table, lens, new, q, dim ** -0.5)
+    for again in range(2):
+        got = _attention(accel, pkg, cache, table, lens, new, raw, ty, dim ** -0.5, always_row0=True)
+        assert np.abs(got - want).max() <= TOL[ty] * 128 * 0.02
+        first = got if again == 0 else first
+    assert np.array_equal(first, got)

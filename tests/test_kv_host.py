@@ -47,3 +47,19 @@ launches = F.fake_launches()
 a.attn_dev(one, batch(1, 1 << 16, 1 << 16, 64), room, 1, 1.0, room)
 assert F.fake_launches() > launches
 """)
+
+
+@pytest.mark.parametrize("nseq,rows,max_rows,max_len", [
+    (2, 8193, 8192, 100000),      # a prompt chunk beside one decode step
+    (9, 8200, 8192, 131072), (65, 8256, 8192, 16384),
+    (4097, 4129, 33, 16384),      # one short chunk beside thousands of decode steps
+    (1000, 1063, 64, 131072), (65, 65, 1, 131072), (1, 2048, 2048, 8192)])
+def test_scratch_of_calls_whose_rows_differ(run, nseq, rows, max_rows, max_len):   # noqa: F811
+    """The attention's scratch goes by the rows whose context is split, not by those beside them."""
+    run(SETUP + """
+F.fake_device_live.restype = C.c_size_t
+wide = pkg.KvCache(1 << 20, 64, 8, 128, room, room, room, room)
+before = F.fake_device_live()
+a.attn_dev(wide, pkg.KvBatch(nseq, room, room, 1 << 12, max_len, row0=room, rows=rows, max_rows=max_rows), room, 32, 0.1, room)
+assert F.fake_device_live() - before <= 257 << 20, (F.fake_device_live() - before) >> 20
+""", nseq=nseq, rows=rows, max_rows=max_rows, max_len=max_len)
