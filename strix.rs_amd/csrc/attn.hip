@@ -92,13 +92,6 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(const AttnArgs A) {
         const bool far = __ballot(fmaxf(fmaxf(key_top[0], key_top[1]), fmaxf(key_top[2], key_top[3])) * unit_top * (32768.0f * 127 * D64) > 0x1p24f) != 0;
         const int plain_hi = __builtin_amdgcn_readfirstlane(far ? -1 : all_hi);   // blocks up to here need no mask
         least = fmaxf(least, least_scale(segment_top<4>(seg)));
-        if ((int)threadIdx.x < n) {
-            // (a value scale of 0 stands for codes of 0; a NaN one is for the rows that see a token of the block)
-            const float scale = seg.vs[threadIdx.x], vs = fmaxf(scale, least);
-            const int e = exponent_of(vs);
-            value[threadIdx.x] = make_float4((float)e, __builtin_amdgcn_logf(vs * pow2(kLift - e)), __builtin_amdgcn_rcpf(vs) * (1.0f / (1 << kLift)), scale);
-        }
-        __syncthreads();
         uint4 kb[PER], vb[PER];
         // this wave's units of a tile: u = wave + 4 j (a last tile's missing block is its first again, and masked)
         auto fetch = [&](int t) {
@@ -268,6 +261,12 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(const AttnArgs A) {
             else weigh(cur, f, base, per_vs, poison, i);
         };
         fetch(0);
+        if ((int)threadIdx.x < n) {
+            // (a value scale of 0 stands for codes of 0; a NaN one is for the rows that see a token of the block)
+            const float scale = seg.vs[threadIdx.x], vs = fmaxf(scale, least);
+            const int e = exponent_of(vs);
+            value[threadIdx.x] = make_float4((float)e, __builtin_amdgcn_logf(vs * pow2(kLift - e)), __builtin_amdgcn_rcpf(vs) * (1.0f / (1 << kLift)), scale);
+        }
         put(0);
         if (tiles > 1) fetch(1);
         __syncthreads();
