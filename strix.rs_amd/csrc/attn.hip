@@ -8,11 +8,12 @@ namespace smx {
 
 namespace {
 
-// The n-th (from 0) of the sequences that are this launch's; -1: there are fewer.
+// The n-th (from 0) of the sequences that are this launch's (or would be, were all their tokens within max_len: looked up by their rows
+// alone); -1: there are fewer.
 __device__ __forceinline__ int nth_sequence(const AttnArgs& A, int n) {
     for (int base = 0; base < A.kv.nseq; base += 64) {   // a wave looks at 64 at a time
         const int s = base + (threadIdx.x & 63);
-        unsigned long long hit = __ballot(s < A.kv.nseq && kv_seq(A.kv, s).n * (int64_t)A.group > A.above);
+        unsigned long long hit = __ballot(s < A.kv.nseq && kv_rows(A.kv, s).n * (int64_t)A.group > A.above);
         const int found = __popcll(hit);
         if (n < found) {
             for (; n > 0; n--) hit &= hit - 1;

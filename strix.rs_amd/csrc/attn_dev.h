@@ -110,11 +110,18 @@ __device__ __forceinline__ float row_max(float v) {
     s = swap16(fmaxf(s.x, s.y));
     return fmaxf(s.x, s.y);
 }
+// Of 16 lanes by DPP moves: neighbours, pairs of them, the half row's mirror, the row's.  (Shuffles go through LDS: four of them one behind
+// the other are a fifth of a microsecond of every workgroup's start.)
+template <int CTRL>
+__device__ __forceinline__ float dpp_max(float v) {
+    return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false)));
+}
 __device__ __forceinline__ float wave_max(float v) {
-    v = row_max(v);
-#pragma unroll
-    for (int o = 1; o < 16; o <<= 1) v = fmaxf(v, __shfl_xor(v, o));
-    return v;
+    v = dpp_max<0xb1>(v);
+    v = dpp_max<0x4e>(v);
+    v = dpp_max<0x141>(v);
+    v = dpp_max<0x140>(v);
+    return row_max(v);
 }
 __device__ __forceinline__ float row_sum(float v) {
     float2 s = swap32(v);

@@ -27,18 +27,21 @@ struct KvArgs {
 struct KvSeq {
     int row, n, len;
 };
-__device__ __forceinline__ KvSeq kv_seq(const KvArgs& a, int s) {
-    const int len = a.len[s];
+// Rows of a sequence from its first one on, without a look at its tokens: within rows and max_rows, and all of them.
+struct KvRows {
+    int row, n, all;
+};
+__device__ __forceinline__ KvRows kv_rows(const KvArgs& a, int s) {
     int r0 = s, r1 = s + 1;   // (without row0 rows is nseq and max_rows 1)
     if (a.row0) { r0 = a.row0[s]; r1 = a.row0[s + 1]; }
-    KvSeq q;
-    q.row = min(max(r0, 0), a.rows);
-    const int all = max(r1, q.row) - q.row, kept = min(all, min(a.rows - q.row, a.max_rows));
-    q.len = max(max(len, 0) - (all - kept), 0);
-    const int over = max(q.len - a.max_len, 0);
-    q.n = max(kept - over, 0);
-    q.len -= over;
-    return q;
+    const int row = min(max(r0, 0), a.rows), all = max(r1, row) - row;
+    return {row, min(all, min(a.rows - row, a.max_rows)), all};
+}
+__device__ __forceinline__ KvSeq kv_seq(const KvArgs& a, int s) {
+    const int len = a.len[s];
+    const KvRows r = kv_rows(a, s);
+    const int held = max(max(len, 0) - (r.all - r.n), 0), over = max(held - a.max_len, 0);
+    return {r.row, max(r.n - over, 0), held - over};
 }
 // Where a head's block `blk` (of SMX_KV_BLOCK tokens) of sequence s is: the page that the table names for it (any number at all), and its index
 // among all blocks of the cache, with page numbers outside the cache clamped into it.
