@@ -283,6 +283,22 @@ def test_rows_beyond_the_call_are_left_out(accel, pkg, new, how):
                 assert np.array_equal(x[ranges[s][0]:ranges[s][1], h], cache.tokens(w, table[s], h, n)[o:])
 
 
+@pytest.mark.parametrize("ty,dim,window,nseq", [("bf16", 256, 1024, 100), ("f32", 128, 900, 150), ("f32", 64, 700, 240), ("bf16", 128, 2040, 112),
+                                                 ("f32", 192, 1000, 80), ("f32", 64, 700, 300), ("bf16", 128, 1000, 260)])
+def test_many_windows(accel, pkg, ty, dim, window, nseq):
+    """Sequences that a window makes alike, in the numbers around a second round of workgroups."""
+    rng = np.random.default_rng(dim + nseq)
+    kv, heads, page, length = 8, 8, 32, 2500
+    cache = _random_cache(rng, page, kv, dim, length)
+    one = R.tables(rng, cache.pages, page, [length])
+    lens = [int(x) for x in rng.integers(1, length + 1, nseq)]
+    q, raw = _queries(rng, ty, nseq, heads, dim)
+    table = np.repeat(one, nseq, 0)
+    want = R.attend(cache, table, lens, [1] * nseq, q, dim ** -0.5, window)
+    got = _attention(accel, pkg, cache, table, lens, [1] * nseq, raw, ty, dim ** -0.5, window=window)
+    assert np.abs(got - want).max() <= TOL[ty] * 128 * 0.02
+
+
 @pytest.mark.parametrize("ty,dim,kv,group,few,chunk", [("f32", 64, 1, 1, [1], 700), ("f32", 128, 2, 4, [1, 1, 0, 1], 300), ("bf16", 64, 1, 8, [1, 5], 200),
                                                        ("f32", 64, 2, 2, [1] * 40, 90), ("bf16", 256, 1, 2, [1, 2, 30], 120)])
 def test_split_contexts_of_decode_steps_beside_chunks(accel, pkg, ty, dim, kv, group, few, chunk):
