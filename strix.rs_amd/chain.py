@@ -125,6 +125,10 @@ class AttentionChain:
         """(stage buffers, output buffer) of layer l."""
         return self.stage[l % len(self.stage)], self.y[l % len(self.y)]
 
+    def _fits(self, rows):
+        if rows > self.rows:
+            raise ValueError(f"{rows} rows, buffers for {self.rows}")
+
     def _project(self, keys, x_dev, rows, outs):
         """rmsnorm of rows of x_dev through the projections `keys`."""
         if rows == 1:
@@ -135,8 +139,7 @@ class AttentionChain:
         """Enqueue all layers for the rows of `batch` on the context's stream (capturable once a call of the same sizes has run); returns the
         device buffer holding the last layer's output."""
         acc, cur = self.acc, x_dev
-        if batch.rows > self.rows:
-            raise ValueError(f"{batch.rows} rows, buffers for {self.rows}")
+        self._fits(batch.rows)
         for l in range(self.layers):
             b, y = self.buffers(l)
             q, k, v, o = self.keys(l)
@@ -152,6 +155,7 @@ class AttentionChain:
 
     def sample(self, y_dev, rows, u_dev, ids_dev, temperature=None, top_k=None, top_p=None, min_p=None, prob=None):
         """Enqueue rmsnorm, the lm_head and the pick of one token for each of `rows` rows of hidden states (device arrays throughout)."""
+        self._fits(rows)
         if not self._project((self.lm_head,), y_dev, rows, (self.logits,)):
             raise RuntimeError("the lm_head is not resident")
         self.acc.sample_dev(self.logits, rows, self.vocab, u_dev, ids_dev, temperature, top_k, top_p, min_p, prob)
