@@ -327,13 +327,14 @@ int smx_attn_dev(smx_ctx* ctx, const smx_kv_cache* cache, const smx_kv_batch* ba
 
 /* ---- one token for each row of logits from given uniform numbers (the reference picks greedily: lm_head_argmax_rows).
  *      Per row, with x the logits (NaN and -inf are never picked; entries equal to a +inf maximum share it) and m their maximum:
- *        temperature T > 0: e_i = exp((x_i - m) / T) in fp32 and the whole-number weight w_i = floor(e_i * 2^40); T <= 0: the
+ *        temperature T > 0: e_i = exp((x_i - m) / T) in fp32 and the whole-number weight w_i = floor(e_i * 2^40); else the
  *                    largest logit, lowest index on equal ones
  *        top_k > 0:  the k first in (logit descending, index ascending) order stay
  *        top_p < 1:  of those, the ones with less than floor(top_p * their total) in front of them in that order stay, and the first
- *        min_p > 0:  of those, the ones with e_i >= min_p stay
+ *        min_p > 0:  of those, the ones with e_i >= min(min_p, 1) stay
  *        the pick is the lowest index whose running total of kept weights (in index order) exceeds floor(u * their total)
- *      All sums are of whole numbers, so a pick does not depend on how the work is split.  u in [0, 1). ---- */
+ *      All sums are of whole numbers, so a pick does not depend on how the work is split; top_p and u times a sum are products of
+ *      64-bit floating point.  u in [0, 1).  A comparison with NaN does not hold: such a filter is off. ---- */
 #define SMX_SAMPLE_MAX_VOCAB 2097152
 typedef struct smx_sample_params { /* device arrays [rows]; NULL: 1, off, off, off for every row */
     const float* temperature;

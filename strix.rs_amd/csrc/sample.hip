@@ -159,7 +159,7 @@ __device__ __forceinline__ Ask ask_of(const SampleArgs& A, int row) {
     q.T = temp_of(T, q.mx);
     q.top_k = A.top_k ? A.top_k[row] : 0;
     q.top_p = A.top_p ? A.top_p[row] : 1.0f;
-    q.min_p = A.min_p ? fminf(A.min_p[row], 1.0f) : 0.0f;
+    q.min_p = A.min_p && A.min_p[row] > 0.0f ? fminf(A.min_p[row], 1.0f) : 0.0f;   // (off where the comparison does not hold: NaN, too)
     const bool k = q.top_k > 0 && q.top_k < A.vocab;
     q.mode = top == 0 ? kNone : !(T > 0.0f) || q.top_k == 1 || q.top_p <= 0.0f ? kGreedy : k ? kTopK : q.top_p < 1.0f ? kTopP : kFree;
     q.bin_T = q.mode == kTopK ? temp_of(1.0f, q.mx) : q.T;
@@ -840,7 +840,7 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(const SampleArgs 
 int launch_sample(smx_ctx* c, const float* logits, size_t rows, size_t vocab, size_t ld, const smx_sample_params* p, const float* u, int32_t* ids, float* prob) {
     SampleArgs A{};
     A.logits = logits; A.ld = (int64_t)ld; A.rows = (int)rows; A.vocab = (int)vocab;
-// (rows that do not all start at 16-byte boundaries may lie up to 3 tokens into their first chunk)
+    // (rows that do not all start at 16-byte boundaries may lie up to 3 tokens into their first chunk)
     const size_t skew = ld % 4 == 0 ? ((uintptr_t)logits >> 2) & 3 : 3;
     A.chunks = (int)((vocab + skew + kChunk - 1) / kChunk);
     if (p) { A.temperature = p->temperature; A.top_k = p->top_k; A.top_p = p->top_p; A.min_p = p->min_p; }
