@@ -463,7 +463,8 @@ int smx_kv_sizes(size_t pages, size_t page_tokens, size_t kv_heads, size_t head_
     if (pages == 0 || page_tokens == 0 || page_tokens % SMX_KV_BLOCK || page_tokens > (size_t(1) << 20) || kv_heads == 0 || kv_heads > 65535 ||
         head_dim == 0 || head_dim % 2 || head_dim > SMX_KV_MAX_HEAD_DIM || pages > (size_t(1) << 31))
         return SMX_ERR_ARG;
-    const size_t blocks = pages * kv_heads * (page_tokens / SMX_KV_BLOCK);
+    const size_t blocks = pages * kv_heads * (page_tokens / SMX_KV_BLOCK);   // < 2^62
+    if (blocks > size_t(1) << 48) return SMX_ERR_ARG;                        // (and their bytes would pass 64 bits)
     *code_bytes = blocks * SMX_KV_BLOCK * ((head_dim + 63) & ~size_t(63));
     *scales = blocks;
     return SMX_OK;

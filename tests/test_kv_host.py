@@ -63,3 +63,11 @@ before = F.fake_device_live()
 a.attn_dev(wide, pkg.KvBatch(nseq, room, room, 1 << 12, max_len, row0=room, rows=rows, max_rows=max_rows), room, 32, 0.1, room)
 assert F.fake_device_live() - before <= 257 << 20, (F.fake_device_live() - before) >> 20
 """, nseq=nseq, rows=rows, max_rows=max_rows, max_len=max_len)
+
+
+def test_cache_whose_bytes_pass_64_bits(pkg):
+    """Sizes that have wrapped would be those of a far smaller cache than the kernels index."""
+    for bad in ((1 << 31, 1 << 20, 65535, 256), (1 << 31, 1 << 20, 8, 128), (1 << 30, 1 << 20, 32, 2)):
+        with pytest.raises(ValueError):
+            pkg.kv_sizes(*bad)
+    assert pkg.kv_sizes(1 << 20, 1 << 15, 8, 256) == (1 << 46, 1 << 33)
