@@ -384,13 +384,13 @@ int launch_tile(smx_ctx* c, const AttnArgs& A, dim3 grid) {
     return SMX_OK;
 }
 // Column tiles of a wave: as many as leave two waves a SIMD their registers (queries and sums are 8 CT DC NT and 16 CT DC of 256).
-// Column tiles of a wave: as many as leave two waves a SIMD their registers (queries and sums are 8 CT DC NT and 16 CT DC of 256).
+// f32 rows of 65..128 channels spill 47 of them: values that are reloaded once a tile or a segment, none between the matrix instructions.
 constexpr int most_wave_tiles(int dc) { return dc <= 2 ? 2 : 1; }
 // Rows of a workgroup in units of 64: 128 (they share each widened byte), or 64 where the work does not fill the chip for long, which makes
 // more workgroups with a shorter way each.  The measure is pairs of a row and a key for each CU; f32 rows of 65..128 channels stay with 64
 // for longer, since 128 of them spill some registers.  us at 64 / 128 rows, 32 heads over 8 key/value heads of 128 channels, bf16 and f32:
-// 32 tokens behind 4000 21 / 29 and 23 / 32, 40 tokens of 4 sequences of 4000 45 / 44 and 54 / 66, 96 of 4 of 16000 249 / 168 and
-// 312 / 261, 512 of 4 of 16000 907 / 649 and 1164 / 1074.
+// 32 tokens behind 4000 21 / 26 and 23 / 30, 40 tokens of 4 sequences of 4000 41 / 40 and 49 / 59, 96 of 4 of 16000 230 / 158 and
+// 296 / 218, 512 of 4 of 16000 882 / 658 and 1135 / 978.
 int tile_waves(const smx_ctx* c, const AttnArgs& A, size_t nseq, size_t rows, size_t reach, bool bf16) {
     const int dc = A.kv.dim64 / 64;
     const double pairs = (double)nseq * A.kv.kv_heads * (double)rows * (double)reach / c->num_cu;

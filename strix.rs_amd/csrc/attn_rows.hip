@@ -20,7 +20,9 @@ namespace {
 constexpr int kJoinInside = 16;      // pieces
 constexpr int kJoinRows = 32;        // rows times pieces
 
-// Sums pass from workgroup to workgroup as words that are atomic at device scope: written to, and read from, where all XCDs see them.
+// Sums pass from workgroup to workgroup as words that are atomic at device scope: written to, and read from, where all XCDs see them, each
+// thread's waited for before the workgroup counts itself.  That such a store has arrived once it has been waited for is the hardware's
+// (gfx950 writes it through its L2); in the language's terms it is no release, which would write the XCD's whole L2 back instead.
 __device__ __forceinline__ void give(float* p, float v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 __device__ __forceinline__ float take(const float* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 __device__ __forceinline__ float row16_max(float v) {   // of 16 lanes
@@ -30,7 +32,7 @@ __device__ __forceinline__ float row16_max(float v) {   // of 16 lanes
 }
 __device__ __forceinline__ float over(float L) { return L > 0.f ? 1.0f / L : L == L ? 0.f : L; }   // (a NaN stays one)
 
-// Waves on a SIMD: what the registers leave.
+// Waves on a SIMD: what the registers leave.  (f32 rows of 193..256 channels spill 24 of them, in front of the loop over blocks and behind it.)
 constexpr int residents(int dc, int ct) { return ct == 2 ? 2 : dc <= 1 ? 4 : dc == 2 ? 3 : 2; }
 
 // Workgroup (head and tile of 16 CT rows, piece of the context, sequence); its four waves (or one) take the piece's blocks in turn, straight

@@ -289,7 +289,8 @@ __global__ __launch_bounds__(kPartThreads) void sample_hist_kernel(const SampleA
         if (w) atomicAdd(&all[i], w);
     }
     // What passes between workgroups is atomic at device scope, performed where all XCDs see it: this thread's additions are
-    // waited for, then the workgroup counts itself; the reads below are atomic too.  (A fence by each wave would write its XCD's L2
+    // waited for, then the workgroup counts itself; the reads below are atomic too.  That an atomic has been performed once it has been
+    // waited for is the hardware's; in the language's terms this is no release.  (A fence by each wave would be one and write its XCD's L2
     // back: 256 rows of 262144 329 us instead of 75.)
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
@@ -682,7 +683,6 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(const SampleArgs 
     unsigned long long *const list = room, *const members = room + kList, *const totals = room + 2 * kList, *const step = totals;
     unsigned long long* const ws = members;         // weights of a chunk
     ulonglong2* const pairs = (ulonglong2*)members; // words and weights of a short list
-    const unsigned long long* sorted = list;
     const int row = blockIdx.x, tid = threadIdx.x;
     const Row r = row_of(A, row);
     const float* x = r.x;
@@ -768,7 +768,6 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(const SampleArgs 
                 last = place(A, q, red, list, n, step, members, found, last, true, cut.above, cut.limit);
             }
             keep = n;
-            sorted = list;
         }
     }
     // the chunks' totals
@@ -787,8 +786,8 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(const SampleArgs 
         }
     } else {
         for (int i = tid; i < keep; i += kThreads) {   // the list's kept tokens (none without a cut)
-            const float e = q.share(of_key(~(unsigned)(sorted[i] >> 32)));
-            if (kept(last, sorted[i]) && e >= q.min_p) atomicAdd(&totals[((unsigned)sorted[i] + r.skew) / kChunk], weight(e));
+            const float e = q.share(of_key(~(unsigned)(list[i] >> 32)));
+            if (kept(last, list[i]) && e >= q.min_p) atomicAdd(&totals[((unsigned)list[i] + r.skew) / kChunk], weight(e));
         }
     }
     __syncthreads();
