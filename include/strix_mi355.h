@@ -277,8 +277,9 @@ typedef struct smx_kv_cache {
 } smx_kv_cache;
 /* The rows of one step: row r of sequence s is the token at position len[s] - n_s + (r - row0[s]), n_s = row0[s + 1] - row0[s];
  * len counts this step's rows in.  len, row0 and table are read on the device when the kernels run, so a captured graph serves
- * every step whose values keep within rows, max_rows and max_len; what they exceed them by is left out.  Tokens whose page number
- * is outside the cache are not stored; for reading, such numbers are clamped into it. */
+ * every step whose values keep within rows, max_rows and max_len; what they exceed them by is left out: a sequence's last rows,
+ * which are neither stored nor attended to nor read back.  Tokens whose page number is outside the cache are not stored; for
+ * reading, such numbers are clamped into it. */
 typedef struct smx_kv_batch {
     size_t nseq;
     const int32_t* len;    /* device [nseq] */
