@@ -91,19 +91,24 @@ class AttentionChain:
         2. smx_kv_append_dev   q and k rotated, k and v into the layer's cache
         3. smx_attn_dev        q over the cache -> o
         4. smx_gemv_dev        quantiser + output projection            o -> y[hidden]
-    and behind the last layer rmsnorm + lm_head and smx_sample_dev on the rows that the caller names.
+    and behind the last layer rmsnorm + lm_head and smx_sample_dev on the rows that the caller names.  enqueue() runs one layer's output straight
+    into the next; a caller with something of its own between them (a residual, the other half of the layer) calls layer() for each.
 
     Each call's rows, lengths and page table are a KvBatch of the caller's, whose device arrays the kernels read when they run: a
     captured decode step (one row for each sequence) serves every later one, with new lengths and pages written in front of it.
 
-    pkg: the package module (its KvCache, KvBatch and Rope); keys(l) -> (q, k, v, o) weight keys of layer l; rows: the most that one
-    call brings.  keep_stages: every layer gets buffers of its own, so that a test can read each stage back."""
+    pkg: the package module (its KvCache, KvBatch and Rope); keys(l) -> (q, k, v, o) weight keys of layer l; norm_w_dev: the rmsnorm weight
+    of every layer and of the end, or a list of layers + 1 of them; rows: the most that one call brings.  keep_stages: every layer gets
+    buffers of its own, so that a test can read each stage back."""
 
     def __init__(self, pkg, acc, layers, hidden, q_heads, kv_heads, head_dim, keys, lm_head, vocab, norm_w_dev, rows, pages, page_tokens, max_pos,
                  rope_base=1e4, window=0, eps=1e-6, keep_stages=False):
         self.pkg, self.acc, self.layers, self.hidden, self.keys = pkg, acc, layers, hidden, keys
         self.q_heads, self.kv_heads, self.head_dim = q_heads, kv_heads, head_dim
-        self.lm_head, self.vocab, self.norm_w_dev, self.rows, self.window, self.eps = lm_head, vocab, norm_w_dev, rows, window, eps
+        self.lm_head, self.vocab, self.rows, self.window, self.eps = lm_head, vocab, rows, window, eps
+        self.norms = list(norm_w_dev) if isinstance(norm_w_dev, (list, tuple)) else [norm_w_dev] * (layers + 1)
+        if len(self.norms) != layers + 1:
+            raise ValueError(f"{len(self.norms)} rmsnorm weights for {layers} layers and the end")
         self._bufs = []
         code_bytes, scales = pkg.kv_sizes(pages, page_tokens, kv_heads, head_dim)
         self.cache = [pkg.KvCache(pages, page_tokens, kv_heads, head_dim, self._alloc(code_bytes), self._alloc(code_bytes), self._alloc(scales * 4),
@@ -129,34 +134,37 @@ class AttentionChain:
         if rows > self.rows:
             raise ValueError(f"{rows} rows, buffers for {self.rows}")
 
-    def _project(self, keys, x_dev, rows, outs):
+    def _project(self, keys, x_dev, norm_w, rows, outs):
         """rmsnorm of rows of x_dev through the projections `keys`."""
         if rows == 1:
-            return self.acc.gemv_fused_dev(list(keys), self.pkg.ACT_RMSNORM, x_dev, self.norm_w_dev, list(outs), self.eps)
-        return all([self.acc.gemm_fused_dev(k, self.pkg.ACT_RMSNORM, x_dev, self.norm_w_dev, rows, y, self.eps) for k, y in zip(keys, outs)])
+            return self.acc.gemv_fused_dev(list(keys), self.pkg.ACT_RMSNORM, x_dev, norm_w, list(outs), self.eps)
+        return all([self.acc.gemm_fused_dev(k, self.pkg.ACT_RMSNORM, x_dev, norm_w, rows, y, self.eps) for k, y in zip(keys, outs)])
+
+    def layer(self, l, x_dev, batch):
+        """Enqueue layer l for the rows of `batch`; returns the device buffer holding its output."""
+        self._fits(batch.rows)
+        acc, (b, y), (q, k, v, o) = self.acc, self.buffers(l), self.keys(l)
+        ok = self._project((q, k, v), x_dev, self.norms[l], batch.rows, (b["q"], b["k"], b["v"]))
+        if ok:
+            acc.kv_append_dev(self.cache[l], batch, b["k"], b["v"], rope=self.rope, q=b["q"], q_heads=self.q_heads, q_out=b["q"])
+            acc.attn_dev(self.cache[l], batch, b["q"], self.q_heads, self.head_dim ** -0.5, b["o"], window=self.window)
+            ok = (acc.gemv_dev if batch.rows <= 32 else acc.gemm_dev)(o, b["o"], batch.rows, y)
+        if not ok:
+            raise RuntimeError(f"layer {l}: a weight of the chain is not resident")
+        return y
 
     def enqueue(self, x_dev, batch):
         """Enqueue all layers for the rows of `batch` on the context's stream (capturable once a call of the same sizes has run); returns the
         device buffer holding the last layer's output."""
-        acc, cur = self.acc, x_dev
-        self._fits(batch.rows)
+        cur = x_dev
         for l in range(self.layers):
-            b, y = self.buffers(l)
-            q, k, v, o = self.keys(l)
-            ok = self._project((q, k, v), cur, batch.rows, (b["q"], b["k"], b["v"]))
-            if ok:
-                acc.kv_append_dev(self.cache[l], batch, b["k"], b["v"], rope=self.rope, q=b["q"], q_heads=self.q_heads, q_out=b["q"])
-                acc.attn_dev(self.cache[l], batch, b["q"], self.q_heads, self.head_dim ** -0.5, b["o"], window=self.window)
-                ok = (acc.gemv_dev if batch.rows <= 32 else acc.gemm_dev)(o, b["o"], batch.rows, y)
-            if not ok:
-                raise RuntimeError(f"layer {l}: a weight of the chain is not resident")
-            cur = y
+            cur = self.layer(l, cur, batch)
         return cur
 
     def sample(self, y_dev, rows, u_dev, ids_dev, temperature=None, top_k=None, top_p=None, min_p=None, prob=None):
         """Enqueue rmsnorm, the lm_head and the pick of one token for each of `rows` rows of hidden states (device arrays throughout)."""
         self._fits(rows)
-        if not self._project((self.lm_head,), y_dev, rows, (self.logits,)):
+        if not self._project((self.lm_head,), y_dev, self.norms[-1], rows, (self.logits,)):
             raise RuntimeError("the lm_head is not resident")
         self.acc.sample_dev(self.logits, rows, self.vocab, u_dev, ids_dev, temperature, top_k, top_p, min_p, prob)
 

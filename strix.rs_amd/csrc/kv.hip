@@ -208,7 +208,7 @@ int touched_blocks(const smx_kv_batch* b) { return b->row0 ? (int)((b->rows + 62
 // partly new, values go by 4 tokens or single bytes, so that nothing is read back unless the scale grew.
 // Bytes bound a prompt chunk (2048 rows of 16 + 16 heads of 256 bf16 channels, 59 MB: 17 us, 20 with the new values in LDS as fp32 and
 // loads asked for one group at a time), the launch and a chain of three loads (the step's arrays, its rows, the page) a decode step
-// (64 rows of 32 + 16 heads of 128: 5.8 us): what does not depend on another load is asked for in front of it.
+// (64 rows of 32 + 16 heads of 128: 6.0 us): what does not depend on another load is asked for in front of it.
 template <bool BF16, bool PAIRS, bool VEC>
 __global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs A) {
 #pragma clang fp contract(off)
