@@ -415,17 +415,18 @@ constexpr size_t kWhole = 384;
 // Contexts up to which (sequence, key/value head) pairs, where they are more than workgroups of four waves have places at once, take a wave
 // each: four waves of a pair have a block or two each and then their sums to put together.  Four waves / one, one row of 32/8 heads of
 // 128 channels: 128 sequences of 50 tokens 15 / 10, of 200 21 / 16, 1000 of 100 98 / 53, of 300 154 / 133, of 500 208 / 203, of 800
-// 307 / 305, of 20..800 188 / 192.
+// 307 / 305, of 20..800 188 / 192.  Where it loses: two column tiles or 64 channels, 350..512 tokens and few more pairs than places (96/4 heads of
+// 64, 564 pairs of 512 tokens 24 / 28), and 256 channels at four times the places (109 / 124).
 // A window makes longer contexts alike too.  There single waves win while four would begin a second round that does not fill the chip (up to
 // 2 rounds), if together they have bytes enough on the way, which goes by pairs times channels (kLoneBytes).  Four waves / one, windows of
 // 512, 1024 and 2048:
 //   16/8 heads of 256, bf16 (512 places): 640 pairs 44/38 73/67 133/126, 768 48/44 85/83 150/149, 1024 58/56 108/107 195/193, 1280 77/71 132/131 239/247
 //   32/8 heads of 128, f32 (768 places): 896 32/26 49/44 99/94, 1024 34/27 54/48 108/100, 1280 38/36 67/67 130/130, 3200 97/99 166/182 310/345
 //   16/8 heads of 192, bf16 (512): 576 35/30 53/48 103/101, 768 40/33 63/58 123/114, 1024 46/41 86/80 150/147
-//   96/4 heads of 128, f32 (512, two column tiles): 576 39/41 52/67 88/122, 896 47/41 65/69 120/130, 1024 48/42 74/69 131/138
+//   96/4 heads of 128, f32 (512, two column tiles: only the shorter windows): 576 39/41 52/67 88/122, 896 47/41 65/69 120/130, 1024 48/42 74/69 131/138
 //   32/4 heads of 64, bf16 (1024): 1280 24/24 36/38 70/78, 1600 27/24 41/39 85/86, 2048 31/27 51/48 105/103
 // and at a window of 4096, which stays with four: 128 channels 183/177, 197/190, 240/250; 256 245/234, 280/281, 373/371.
-constexpr size_t kLone = 512, kLoneWindow = 2112, kLoneBytes = 7 << 14;
+constexpr size_t kLone = 512, kLoneWindow = 2112, kLoneWindowTwo = 576, kLoneBytes = 7 << 14;
 // Tokens of 128 channels of a piece, however many sequences there are: the call knows the longest only, and one long sequence among short ones
 // would keep a few workgroups busy for long after the others.  One row each of 64 sequences of 500 tokens and one of 131072: 145 us, without
 // 1163; 64 of 33..32768 430 / 462; where all are alike it costs a little: 64 of 16384 394 / 370.
@@ -458,7 +459,7 @@ int attend(smx_ctx* c, AttnArgs A, size_t nseq, size_t rows, size_t reach, bool 
     split = std::max(split, span * A.kv.dim64 / 128 / kLongest);
     split = std::min({split, std::max<size_t>(1, kMostSums / (kept * each)), (size_t)kMaxPieces});
     const size_t places = cus * rows_residents(A.kv.dim64, A.tile_rows);
-    const bool alike = A.window > 0 && span <= kLoneWindow && A.tile_rows == 16 && groups <= 2 * places && groups * A.kv.dim64 >= kLoneBytes;
+    const bool alike = A.window > 0 && span <= (A.tile_rows == 16 ? kLoneWindow : kLoneWindowTwo) && groups <= 2 * places && groups * A.kv.dim64 >= kLoneBytes;
     A.lone = few && groups > places && (span <= kLone || alike);
     const size_t piece = std::max<size_t>(((span + split - 1) / split + 127) & ~size_t(127), 128);
     A.piece = (int)std::min<size_t>(piece, size_t(1) << 30);

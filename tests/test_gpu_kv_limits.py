@@ -280,12 +280,12 @@ def test_rows_beyond_the_call_are_left_out(accel, pkg, new, how):
                 assert np.array_equal(x[ranges[s][0]:ranges[s][1], h], cache.tokens(w, table[s], h, n)[o:])
 
 
-@pytest.mark.parametrize("ty,dim,window,nseq", [("bf16", 256, 1024, 100), ("f32", 128, 900, 150), ("f32", 64, 700, 240), ("bf16", 128, 2040, 112),
-                                                 ("f32", 192, 1000, 80), ("f32", 64, 700, 300), ("bf16", 128, 1000, 260)])
-def test_many_windows(accel, pkg, ty, dim, window, nseq):
+@pytest.mark.parametrize("ty,dim,window,nseq,kv,heads", [("bf16", 256, 1024, 100, 8, 8), ("f32", 128, 900, 150, 8, 8), ("f32", 64, 700, 240, 8, 8), ("bf16", 128, 2040, 112, 8, 8),
+                                                 ("f32", 192, 1000, 80, 8, 8), ("f32", 64, 700, 300, 8, 8), ("bf16", 128, 1000, 260, 8, 8), ("f32", 128, 500, 240, 4, 68)])
+def test_many_windows(accel, pkg, ty, dim, window, nseq, kv, heads):
     """Sequences that a window makes alike, in the numbers around a second round of workgroups."""
     rng = np.random.default_rng(dim + nseq)
-    kv, heads, page, length = 8, 8, 32, 2500
+    page, length = 32, 2500
     cache = _random_cache(rng, page, kv, dim, length)
     one = R.tables(rng, cache.pages, page, [length])
     lens = [int(x) for x in rng.integers(1, length + 1, nseq)]
